@@ -1,0 +1,719 @@
+// masked_attention: the tokens of a prompt attend to each other, with the
+// masks and score rules of language models (operatorlib/lm_c.h).
+//
+// Per (batch, query head) the online recurrence of the flash kernels:
+// m' = max(m, x), O^T' = O^T 2^(m - m') + V^T P^T, no S x S matrix. The tiles
+// and lane layout are attention.hip's: S^T = K Q^T and O^T += V^T P^T on
+// v_mfma_f32_16x16x32_f16 (fp32: 16x16x4), so that the S^T accumulators of a
+// lane are its part of the P^T operand; K and V tiles copied global -> LDS by
+// buffer loads with the lds modifier, two stages, 16-byte chunks XOR-swizzled;
+// V^T read with ds_read_b64_tr_b16; fp16 row sums on the matrix cores; the
+// running max moves only by more than kLazyLog2.
+//
+// What the rules add:
+//   * Visibility of key j to query i, without documents, is j < prefix or
+//     lo(i) <= j <= hi(i): two compares. lo and hi come from causal and window.
+//   * A query block visits the key tiles of the prefix and of
+//     [lo(first row), hi(last row)] only. With documents it first marks, per
+//     64 keys, whether any of them is in the block's span of documents, and
+//     whether all of them and all rows are one document; unmarked tiles are
+//     skipped, tiles of one document inside the bounds need no mask.
+//   * A wavefront applies the mask only in tiles that some of its rows see in
+//     part.
+//   * A hidden key's probability is 0, but 0 x infinity is NaN: if a block's O
+//     ends with a NaN, the block runs again and keeps, in the tiles that are
+//     seen in part, non-finite values out of the matrix product; they are
+//     added to the rows that see them. Blocks without a NaN pay one test.
+
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+#include <cmath>
+#include <cstddef>
+#include <cstdint>
+#include <type_traits>
+
+#include "attention_tiles.hpp"
+#include "common.hpp"
+#include "lm_validate.hpp"
+#include "operatorlib/lm_c.h"
+#include "scores.hpp"
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+#define OPL_LDS __attribute__((address_space(3)))
+
+constexpr int kXcds = 8;
+constexpr int kRowsPerWave = 32;
+// Headroom (log2 units) the running max may lag the true max by.
+constexpr float kLazyLog2 = 8.0f;
+// Workgroup slots of an XCD that a causal launch balances (attention.hip).
+constexpr int kCausalGroupSlots = 64;
+constexpr int kMarkWords = opl::kMaxMaskedSequence / 64 / 32;  // a bit per 64 keys
+
+template <typename T>
+struct MaskedArgs {
+  const T* q;
+  const T* k;
+  const T* v;
+  T* out;
+  opl::MaskedStrides qs, ks, vs, os;
+  const float* slopes;
+  const std::int32_t* documents;
+  const std::int32_t* prefixes;
+  int bh, q_heads, group, S, dm, causal, window;
+  opl::ScoreRules rules;
+};
+
+template <typename T, int D, int kGroups, int kW, int kTileKeys>
+constexpr int kMinWavesPerSimd =
+    2 * kGroups * opl::Layout<T, D, kTileKeys>::kStage > 80 * 1024 && kGroups * kW == 4 ? 1 : 2;
+
+// kW wavefronts of 32 query rows share the tiles of a group; kGroups groups
+// (small grids) take every kGroups-th tile of the same rows and join at the
+// end. kRules: scores are capped or biased (else they are only scaled).
+template <typename T, int D, int kGroups, int kW, int kTileKeys, bool kRules>
+__global__ __launch_bounds__(kW * opl::kWaveSize * kGroups)
+__attribute__((amdgpu_waves_per_eu(kMinWavesPerSimd<T, D, kGroups, kW, kTileKeys>, 2)))
+void masked_attention_kernel(const MaskedArgs<T> a) {
+  using L = opl::Layout<T, D, kTileKeys>;
+  constexpr bool kHalf = L::kSize == 2;
+  using Frag = typename std::conditional<kHalf, half8, floatx4>::type;
+  constexpr int kRows = kW * kRowsPerWave;
+  constexpr int kThreads = kW * kGroups * opl::kWaveSize;
+  constexpr int kCopies = L::kTile / 16 / (kW * opl::kWaveSize);
+  constexpr int kArray = kGroups * L::kStage;
+  __shared__ __attribute__((aligned(1024))) unsigned char stage0[kArray];
+  __shared__ __attribute__((aligned(1024))) unsigned char stage1[kArray];
+  __shared__ unsigned marked[kMarkWords];  // some key of the 64 may be visible
+  __shared__ unsigned single[kMarkWords];  // all rows and all 64 keys are one document
+  __shared__ int again;
+
+  // ---- which rows of which head: XCD x takes a contiguous range of the work,
+  // heads in order (the query heads of a key head follow each other), heaviest
+  // block of a causal head first, groups of heads interleaved where a head has
+  // few blocks (attention.hip).
+  const int S = a.S;
+  const int q_blocks = (S + kRows - 1) / kRows;
+  const int total = q_blocks * a.bh;
+  const int per_xcd = (total + kXcds - 1) / kXcds;
+  const int w = static_cast<int>(blockIdx.x % kXcds) * per_xcd + static_cast<int>(blockIdx.x / kXcds);
+  if (w >= total) return;
+  int bh = w / q_blocks;
+  int qb = q_blocks - 1 - w % q_blocks;
+  if (a.causal) {
+    const int g = max(1, kCausalGroupSlots / q_blocks);
+    if (g > 1) {
+      const int first = w / (g * q_blocks) * g;
+      const int heads = min(g, a.bh - first);
+      const int r = w - first * q_blocks;
+      bh = first + r % heads;
+      qb = q_blocks - 1 - r / heads;
+    }
+  }
+  const int batch = bh / a.q_heads;
+  const int head = bh % a.q_heads;
+  const int q0 = qb * kRows;
+  const int lane = threadIdx.x % opl::kWaveSize;
+  const int wave = (threadIdx.x / opl::kWaveSize) % kW;
+  const int group = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / opl::kWaveSize / kW);
+  unsigned char* const st0 = stage0 + group * L::kStage;
+  unsigned char* const st1 = stage1 + group * L::kStage;
+  const int col = lane % 16;
+  const int quad = lane / 16;
+  const int wave_row0 = q0 + wave * kRowsPerWave;
+  const int dm = a.dm;
+  const T* qh = a.q + batch * a.qs.batch + head * a.qs.head;
+  const T* kh = a.k + batch * a.ks.batch + (head / a.group) * a.ks.head;
+  const T* vh = a.v + batch * a.vs.batch + (head / a.group) * a.vs.head;
+  const std::int32_t* docs =
+      a.documents != nullptr ? a.documents + static_cast<std::int64_t>(batch) * S : nullptr;
+  const int prefix = a.prefixes != nullptr ? min(max(a.prefixes[batch], 0), S) : 0;
+  // Bounds of the keys that row i sees outside the prefix. (window up to
+  // 2^31 - 1: i - window + 1 cannot underflow, and the sum is taken against S - i.)
+  auto low = [&](int i) { return a.window > 0 ? max(0, i - a.window + 1) : 0; };
+  auto high = [&](int i) {
+    if (a.causal) return min(i, S - 1);
+    return a.window > 0 && a.window < S - i ? i + a.window - 1 : S - 1;
+  };
+
+  // ---- the tiles that the block visits
+  const int last_row = min(q0 + kRows, S) - 1;
+  const int prefix_tiles = (prefix + kTileKeys - 1) / kTileKeys;
+  const int from_tile = low(q0) / kTileKeys;
+  const int end_tile = max(prefix_tiles, high(last_row) / kTileKeys + 1);
+  if (docs != nullptr) {
+    // The block's documents: the least and greatest id of its rows.
+    int least = 0x7fffffff, most = -1;
+    bool all = true;
+    for (int i = q0 + lane; i <= last_row; i += opl::kWaveSize) {
+      const int id = docs[i];
+      if (id >= 0) {
+        least = min(least, id);
+        most = max(most, id);
+      } else {
+        all = false;
+      }
+    }
+#pragma unroll
+    for (int step = 1; step < opl::kWaveSize; step *= 2) {
+      least = min(least, __shfl_xor(least, step));
+      most = max(most, __shfl_xor(most, step));
+    }
+    const bool one = __builtin_amdgcn_ballot_w64(!all) == 0 && least == most;
+    const int chunks = (end_tile * kTileKeys + 63) / 64;
+    for (int word = threadIdx.x / opl::kWaveSize; word * 32 < chunks; word += kThreads / opl::kWaveSize) {
+      unsigned some = 0, same = 0;
+#pragma unroll 8
+      for (int bit = 0; bit < 32; ++bit) {
+        const int key = (word * 32 + bit) * 64 + lane;
+        const int id = key < S ? docs[key] : -1;
+        if (__builtin_amdgcn_ballot_w64(id >= least && id <= most) != 0) some |= 1u << bit;
+        if (one && __builtin_amdgcn_ballot_w64(id != least) == 0) same |= 1u << bit;
+      }
+      if (lane == 0) {
+        marked[word] = some;
+        single[word] = same;
+      }
+    }
+    __syncthreads();
+  }
+  // The first visited tile from t on (end_tile: none left). Wave-uniform.
+  auto visit = [&](int t) {
+    if (t >= prefix_tiles && t < from_tile) t = from_tile;
+    if (docs != nullptr) {
+      while (t < end_tile) {
+        const int bit = t * kTileKeys / 64;
+        const unsigned rest = __builtin_amdgcn_readfirstlane(marked[bit / 32]) >> (bit % 32);
+        if (rest & 1) break;
+        // the next marked 64 keys of this word, or the next word
+        const int skip = rest != 0 ? __builtin_ctz(rest) : 32 - bit % 32;
+        t = (bit + skip) * 64 / kTileKeys;
+        if (t >= prefix_tiles && t < from_tile) t = from_tile;
+      }
+    }
+    return min(t, end_tile);
+  };
+
+  // ---- Q^T operand, masks of the lane's rows
+  Frag qf[2][L::kSteps];
+  int row_lo[2], row_span[2], row_doc[2];
+#pragma unroll
+  for (int qc = 0; qc < 2; ++qc) {
+    const int i = min(wave_row0 + 16 * qc + col, S - 1);
+#pragma unroll
+    for (int c = 0; c < L::kSteps; ++c) {
+      const int dim = L::kSubK * c + L::kElems * quad;
+      qf[qc][c] = *reinterpret_cast<const Frag*>(qh + i * a.qs.token + (dim < dm ? dim : 0));
+      if (dim >= dm) qf[qc][c] = Frag{};
+    }
+    row_lo[qc] = low(i);
+    row_span[qc] = high(i) - row_lo[qc];
+    row_doc[qc] = docs != nullptr ? docs[i] : 0;
+  }
+  const float slope = kRules && a.slopes != nullptr ? a.slopes[head] * opl::kLog2e : 0.0f;
+
+  // ---- copies of a tile: byte offset of the lane's chunks, swizzled
+  constexpr int kNoData = static_cast<int>(0x80000000u);
+  int k_src[kCopies], v_src[kCopies];
+#pragma unroll
+  for (int j = 0; j < kCopies; ++j) {
+    const int slot = (wave * kCopies + j) * 64 + lane;
+    const int row = slot / L::kChunks;
+    const int phys = slot % L::kChunks;
+    const int kd = L::kElems * (phys ^ L::swizzle_k(row));
+    const int vd = L::kElems * (phys ^ L::swizzle_v(row));
+    k_src[j] = kd < dm ? (row * static_cast<int>(a.ks.token) + kd) * L::kSize : kNoData;
+    v_src[j] = vd < dm ? (row * static_cast<int>(a.vs.token) + vd) * L::kSize : kNoData;
+  }
+  const unsigned k_bytes = static_cast<unsigned>((S - 1) * a.ks.token + dm) * L::kSize;
+  const unsigned v_bytes = static_cast<unsigned>((S - 1) * a.vs.token + dm) * L::kSize;
+  const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+  auto issue = [&](unsigned char* st, int key0) {  // key0 < S: the range stays positive
+    const std::size_t k_at = static_cast<std::size_t>(key0) * a.ks.token;
+    const std::size_t v_at = static_cast<std::size_t>(key0) * a.vs.token;
+    const unsigned k_rest = k_bytes - static_cast<unsigned>(k_at) * L::kSize;
+    const unsigned v_rest = v_bytes - static_cast<unsigned>(v_at) * L::kSize;
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j)
+      opl::buffer_copy16_lds(kh + k_at, k_rest, st + (wave_s * kCopies + j) * 1024, k_src[j]);
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j)
+      opl::buffer_copy16_lds(vh + v_at, v_rest, st + L::kTile + (wave_s * kCopies + j) * 1024, v_src[j]);
+  };
+  int k_off[L::kSteps];
+#pragma unroll
+  for (int c = 0; c < L::kSteps; ++c)
+    k_off[c] = col * L::kRowBytes + (((4 * c + quad) ^ L::swizzle_k(col)) * 16);
+  int v_base[L::kDBlocks];
+#pragma unroll
+  for (int db = 0; db < L::kDBlocks; ++db) {
+    if constexpr (kHalf) {
+      const int row = 4 * quad + col / 4;
+      const int d = 16 * db + 4 * (col % 4);
+      v_base[db] = L::kTile + row * L::kRowBytes + (((d >> 3) ^ L::swizzle_v(row)) * 16) + (d & 7) * 2;
+    } else {
+      const int row = 4 * quad;
+      const int d = 16 * db + col;
+      v_base[db] = L::kTile + row * L::kRowBytes + (((d >> 2) ^ L::swizzle_v(row)) * 16) + (d & 3) * 4;
+    }
+  }
+
+  // ---- state: lane l holds query 16 qc + col, dims 16 db + 4 quad + e of O^T
+  floatx4 o[2][L::kDBlocks];
+  float row_max[2], move_above[2], lane_sum[2];
+  floatx4 sums[2];
+  half8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
+  const float scale = kRules ? 1.0f : a.rules.scale;
+  const float inv_scale = 1.0f / scale;
+
+  auto run = [&](auto exact_tag) {
+    constexpr bool kExact = decltype(exact_tag)::value;
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc) {
+#pragma unroll
+      for (int db = 0; db < L::kDBlocks; ++db) o[qc][db] = floatx4{0, 0, 0, 0};
+      sums[qc] = floatx4{0, 0, 0, 0};
+      lane_sum[qc] = 0.0f;
+      row_max[qc] = -FLT_MAX;
+      move_above[qc] = -INFINITY;
+    }
+
+    auto body = [&](const unsigned char* cur, int key0, auto masked_tag) {
+      constexpr bool kMasked = decltype(masked_tag)::value;
+      constexpr int kHalves = kTileKeys / 32;
+      floatx4 s[kHalves][2][2];  // [32 keys][16 keys][qc]
+      int ids[kHalves][2][4];
+      if (kMasked && docs != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kHalves; ++j)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              ids[j][kb][e] = docs[min(key0 + 32 * j + 16 * kb + 4 * quad + e, S - 1)];
+      }
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int j = 0; j < kHalves; ++j) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int qc = 0; qc < 2; ++qc) s[j][kb][qc] = floatx4{0, 0, 0, 0};
+        if constexpr (kHalf) {
+          half8 f[2][L::kSteps];
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int c = 0; c < L::kSteps; ++c)
+              f[kb][c] = *reinterpret_cast<const half8*>(cur + k_off[c] + (32 * j + 16 * kb) * L::kRowBytes);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int c = 0; c < L::kSteps; ++c)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int qc = 0; qc < 2; ++qc)
+                s[j][kb][qc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[kb][c], qf[qc][c], s[j][kb][qc], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int c = 0; c < L::kSteps; ++c) {
+            floatx4 f[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+              f[kb] = *reinterpret_cast<const floatx4*>(cur + k_off[c] + (32 * j + 16 * kb) * L::kRowBytes);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int qc = 0; qc < 2; ++qc)
+                  s[j][kb][qc] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[kb][e], qf[qc][c][e], s[j][kb][qc], 0, 0, 0);
+          }
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      float raw[2];
+#pragma unroll
+      for (int qc = 0; qc < 2; ++qc) raw[qc] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kHalves; ++j)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + 32 * j + 16 * kb + 4 * quad + e;
+              float x = s[j][kb][qc][e];
+              if constexpr (kRules) {
+                x = a.rules.template log2_score<!kHalf>(x);
+                if (a.slopes != nullptr)
+                  x -= slope * fabsf(static_cast<float>(wave_row0 + 16 * qc + col - key));
+              }
+              if constexpr (kMasked) {
+                bool seen = static_cast<unsigned>(key - row_lo[qc]) <= static_cast<unsigned>(row_span[qc]) ||
+                            key < prefix;
+                if (docs != nullptr) seen = seen && ids[j][kb][e] == row_doc[qc] && row_doc[qc] >= 0;
+                if (!seen) x = -INFINITY;
+              }
+              s[j][kb][qc][e] = x;
+              raw[qc] = __builtin_elementwise_maximum(raw[qc], x);
+            }
+      if (__builtin_amdgcn_ballot_w64(raw[0] > move_above[0] || raw[1] > move_above[1]) != 0) {
+#pragma unroll
+        for (int qc = 0; qc < 2; ++qc) {
+          const float top = opl::max_lane_xor32(opl::combine_xor16_f32<opl::MaxOp>(raw[qc]));
+          const float new_max = fmaxf(row_max[qc], top * scale);
+          const float alpha = opl::fast_exp2(row_max[qc] - new_max);
+          row_max[qc] = new_max;
+          move_above[qc] = (new_max + kLazyLog2) * inv_scale;
+          if constexpr (kHalf) sums[qc] *= alpha;
+          else lane_sum[qc] *= alpha;
+#pragma unroll
+          for (int db = 0; db < L::kDBlocks; ++db) o[qc][db] *= alpha;
+        }
+      }
+      // Exact pass, tile seen in part: are there non-finite values in it?
+      bool poisoned = false;
+      if constexpr (kExact && kMasked) {
+        bool bad = false;
+        for (int i = lane; i < L::kTile / 4; i += opl::kWaveSize) {
+          if constexpr (kHalf) {
+            const unsigned u = *reinterpret_cast<const unsigned*>(cur + L::kTile + 4 * i);
+            bad |= (((u & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
+          } else {
+            const unsigned u = *reinterpret_cast<const unsigned*>(cur + L::kTile + 4 * i);
+            bad |= (u & 0x7f800000u) == 0x7f800000u;
+          }
+        }
+        poisoned = __builtin_amdgcn_ballot_w64(bad) != 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kHalves; ++j) {
+        const int rows = 32 * j * L::kRowBytes;
+        if constexpr (kHalf) {
+          half8 p[2];
+#pragma unroll
+          for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                p[qc][4 * kb + e] = static_cast<_Float16>(opl::fast_exp2(
+                    kRules ? s[j][kb][qc][e] - row_max[qc] : fmaf(s[j][kb][qc][e], scale, -row_max[qc])));
+#pragma unroll
+          for (int db = 0; db < L::kDBlocks; ++db) {
+            const fp16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16((OPL_LDS fp16x4*)(cur + v_base[db] + rows));
+            const fp16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                (OPL_LDS fp16x4*)(cur + v_base[db] + rows + 16 * L::kRowBytes));
+            half8 f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f[e] = lo4[e];
+              f[4 + e] = hi4[e];
+            }
+            if constexpr (kExact && kMasked) {
+              if (poisoned) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (!(fabsf(static_cast<float>(f[e])) < INFINITY)) f[e] = static_cast<_Float16>(0.0f);
+              }
+            }
+#pragma unroll
+            for (int qc = 0; qc < 2; ++qc)
+              o[qc][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[qc], o[qc][db], 0, 0, 0);
+          }
+#pragma unroll
+          for (int qc = 0; qc < 2; ++qc)
+            sums[qc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[qc], sums[qc], 0, 0, 0);
+        } else {
+          float p[2][2][4];
+#pragma unroll
+          for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                p[qc][kb][e] = opl::fast_exp2(
+                    kRules ? s[j][kb][qc][e] - row_max[qc] : fmaf(s[j][kb][qc][e], scale, -row_max[qc]));
+                lane_sum[qc] += p[qc][kb][e];
+              }
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float f[L::kDBlocks];
+#pragma unroll
+              for (int db = 0; db < L::kDBlocks; ++db) {
+                f[db] = *reinterpret_cast<const float*>(cur + v_base[db] + rows + (16 * kb + e) * L::kRowBytes);
+                if constexpr (kExact && kMasked) {
+                  if (poisoned && !(fabsf(f[db]) < INFINITY)) f[db] = 0.0f;
+                }
+              }
+#pragma unroll
+              for (int db = 0; db < L::kDBlocks; ++db)
+#pragma unroll
+                for (int qc = 0; qc < 2; ++qc)
+                  o[qc][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[db], p[qc][kb][e], o[qc][db], 0, 0, 0);
+            }
+        }
+      }
+      // The non-finite values go to the rows that see their keys.
+      if constexpr (kExact && kMasked) {
+        if (poisoned) {
+          for (int r = 0; r < kTileKeys && key0 + r < S; ++r) {
+            const int key = key0 + r;
+            const int id = docs != nullptr ? docs[key] : 0;
+#pragma unroll
+            for (int qc = 0; qc < 2; ++qc) {
+              bool seen = static_cast<unsigned>(key - row_lo[qc]) <= static_cast<unsigned>(row_span[qc]) || key < prefix;
+              if (docs != nullptr) seen = seen && id == row_doc[qc] && row_doc[qc] >= 0;
+#pragma unroll
+              for (int db = 0; db < L::kDBlocks; ++db)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int d = 16 * db + 4 * quad + e;
+                  const float x = static_cast<float>(*reinterpret_cast<const T*>(
+                      cur + L::kTile + r * L::kRowBytes +
+                      (((d / L::kElems) ^ L::swizzle_v(r)) * 16) + (d % L::kElems) * L::kSize));
+                  if (seen && !(fabsf(x) < INFINITY)) o[qc][db][e] += x;
+                }
+            }
+          }
+        }
+      }
+    };
+
+    // One tile: `t` is in cur; the copy of the group's next tile goes to nxt.
+    auto advance = [&](int t) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) t = visit(t + 1);
+      return t;
+    };
+    auto tile = [&](const unsigned char* cur, unsigned char* nxt, int t) {
+      const int after = t < end_tile ? advance(t) : end_tile;
+      if (after < end_tile) issue(nxt, after * kTileKeys);
+      __builtin_amdgcn_sched_barrier(0);
+      const int key0 = t * kTileKeys;
+      const int key1 = key0 + kTileKeys - 1;
+      const int row0 = wave_row0, row1 = min(wave_row0 + kRowsPerWave, S) - 1;
+      if (t < end_tile && row0 < S &&
+          (key0 < prefix || (key1 >= low(row0) && key0 <= high(row1)))) {
+        bool whole = key1 < prefix || (key0 >= low(row1) && key1 <= high(row0));
+        if (docs != nullptr) {
+          const int bit = key0 / 64;
+          whole = whole && ((single[bit / 32] >> (bit % 32)) & 1) != 0;
+        }
+        if (__builtin_amdgcn_readfirstlane(whole))
+          body(cur, key0, std::false_type{});
+        else
+          body(cur, key0, std::true_type{});
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      if constexpr (kW == 1) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        __syncthreads();
+      }
+      return after;
+    };
+    int t = visit(0);
+    for (int g = 0; g < group; ++g) t = visit(t + 1);
+    if (t < end_tile) issue(st0, t * kTileKeys);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if constexpr (kGroups == 1 || kW == 1) {
+      while (t < end_tile) {  // uniform over the wavefronts that meet at the barrier
+        t = tile(st0, st1, t);
+        if (t >= end_tile) break;
+        t = tile(st1, st0, t);
+      }
+    } else {
+      // Groups of more wavefronts meet at the workgroup's barrier: all run as
+      // many steps as the first group, which has the most tiles.
+      int lead = visit(0);
+      while (lead < end_tile) {
+        lead = advance(lead);
+        t = tile(st0, st1, t);
+        if (lead >= end_tile) break;
+        lead = advance(lead);
+        t = tile(st1, st0, t);
+      }
+    }
+    __syncthreads();  // every stage is free
+  };
+
+  run(std::false_type{});
+  {
+    bool bad = false;
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+      for (int db = 0; db < L::kDBlocks; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= o[qc][db][e] != o[qc][db][e];
+    if (threadIdx.x == 0) again = 0;
+    __syncthreads();
+    if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) again = 1;
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(again)) run(std::true_type{});
+  }
+
+  // ---- join the groups, normalise, store whole rows through LDS
+  float row_sum[2], coef[2];
+#pragma unroll
+  for (int qc = 0; qc < 2; ++qc)
+    row_sum[qc] = kHalf ? sums[qc][0]
+                        : opl::sum_lane_xor32(opl::combine_xor16_f32<opl::SumOp>(lane_sum[qc]));
+  auto inverse = [](float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; };
+  if constexpr (kGroups > 1) {
+    constexpr int kSlots = kThreads;
+    float* const xs = reinterpret_cast<float*>(stage0);
+    const int slot = threadIdx.x;
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc) {
+      xs[qc * kSlots + slot] = row_max[qc];
+      xs[(2 + qc) * kSlots + slot] = row_sum[qc];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc) {
+      float m = -FLT_MAX, l = 0.0f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        m = fmaxf(m, xs[qc * kSlots + (g * kW + wave) * opl::kWaveSize + lane]);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int sl = (g * kW + wave) * opl::kWaveSize + lane;
+        l += xs[(2 + qc) * kSlots + sl] * opl::fast_exp2(xs[qc * kSlots + sl] - m);
+      }
+      coef[qc] = opl::fast_exp2(row_max[qc] - m) * inverse(l);
+    }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc) coef[qc] = inverse(row_sum[qc]);
+  }
+  constexpr int kBlockBytes = kRowsPerWave * D * 4;
+  constexpr int kPerArray = kArray / kBlockBytes;
+  static_assert(kPerArray >= 1 && kGroups * kW <= 2 * kPerArray, "blocks fit the stage arrays");
+  auto block = [&](int index) -> floatx4* {
+    return reinterpret_cast<floatx4*>(index < kPerArray ? stage0 + index * kBlockBytes
+                                                        : stage1 + (index - kPerArray) * kBlockBytes);
+  };
+  constexpr int kQuads = D / 4;  // groups of 4 dims in a row
+  {
+    floatx4* const to = block(group * kW + wave);
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+      for (int db = 0; db < L::kDBlocks; ++db) {
+        const int r = 16 * qc + col;
+        to[r * kQuads + ((4 * db + quad) ^ (r % kQuads))] = o[qc][db] * coef[qc];
+      }
+  }
+  __syncthreads();
+  // Each wavefront stores 32 / kGroups rows of its block's kGroups copies.
+  constexpr int kLanes = kQuads;                       // lanes per row
+  constexpr int kRowsPerStore = opl::kWaveSize / kLanes;
+  constexpr int kWaveRows = kRowsPerWave / kGroups;
+  typedef T Out __attribute__((ext_vector_type(4)));
+  const int v = group * kW + wave;
+  const int bw = v / kGroups;
+  const int cc = lane % kLanes;
+  T* const obase = a.out + batch * a.os.batch + head * a.os.head;
+#pragma unroll
+  for (int i = 0; i < kWaveRows / kRowsPerStore; ++i) {
+    const int row = (v % kGroups) * kWaveRows + kRowsPerStore * i + lane / kLanes;
+    const int at = row * kQuads + (cc ^ (row % kQuads));
+    floatx4 x = block(bw)[at];
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) x += block(g * kW + bw)[at];
+    const int token = q0 + kRowsPerWave * bw + row;
+    if (token < S && 4 * cc < dm) {
+      Out y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(x[e]);
+      *reinterpret_cast<Out*>(obase + token * a.os.token + 4 * cc) = y;
+    }
+  }
+}
+
+template <typename T, int D, int kGroups, int kW, int kTileKeys>
+hipError_t launch(const MaskedArgs<T>& a, hipStream_t stream) {
+  constexpr int kRows = kRowsPerWave * kW;
+  const long long blocks = (a.S + kRows - 1LL) / kRows * a.bh;
+  const dim3 grid(static_cast<unsigned>((blocks + kXcds - 1) / kXcds * kXcds));
+  const dim3 block(kGroups * kW * opl::kWaveSize);
+  if (a.rules.cap != 0.0f || a.slopes != nullptr)
+    masked_attention_kernel<T, D, kGroups, kW, kTileKeys, true><<<grid, block, 0, stream>>>(a);
+  else
+    masked_attention_kernel<T, D, kGroups, kW, kTileKeys, false><<<grid, block, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+int masked_entry(MaskedArgs<T> a, int batch, int kv_heads, float scale, float softcap,
+                 void* stream_handle) {
+  const opl::MaskedShape shape = {batch, a.q_heads, kv_heads, a.S, a.dm};
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.out == nullptr ||
+      !opl::masked_shape_ok(shape, sizeof(T)) || !opl::score_rules_ok(scale, a.window, softcap) ||
+      !opl::masked_strides_ok(a.q, a.qs, shape, sizeof(T)) ||
+      !opl::masked_strides_ok(a.k, a.ks, shape, sizeof(T)) ||
+      !opl::masked_strides_ok(a.v, a.vs, shape, sizeof(T)) ||
+      !opl::masked_strides_ok(a.out, a.os, shape, sizeof(T)))
+    return hipErrorInvalidValue;
+  a.bh = batch * a.q_heads;
+  a.group = a.q_heads / kv_heads;
+  a.rules = opl::ScoreRules::of(scale, softcap);
+  const hipStream_t stream = static_cast<hipStream_t>(stream_handle);
+  // Blocks of 32 rows on four key groups while their grid is one round of the
+  // 256 CUs; else 128 rows per workgroup.
+  const bool few = (a.S + 31LL) / 32 * a.bh <= 256;
+  const bool wide = a.dm > 64;
+  if constexpr (sizeof(T) == 2) {
+    if (few) return wide ? launch<T, 128, 4, 1, 32>(a, stream) : launch<T, 64, 4, 1, 32>(a, stream);
+    return wide ? launch<T, 128, 1, 4, 64>(a, stream) : launch<T, 64, 1, 4, 64>(a, stream);
+  } else {
+    if (few) return wide ? launch<T, 128, 2, 2, 32>(a, stream) : launch<T, 64, 4, 1, 32>(a, stream);
+    return wide ? launch<T, 128, 1, 4, 32>(a, stream) : launch<T, 64, 1, 4, 32>(a, stream);
+  }
+}
+
+opl::MaskedStrides of(operatorlib_strides_t s) { return {s.batch, s.head, s.token}; }
+
+}  // namespace
+
+extern "C" int operatorlib_masked_attention_f16(
+    const operatorlib_half_t* q, operatorlib_strides_t q_strides, const operatorlib_half_t* k,
+    operatorlib_strides_t k_strides, const operatorlib_half_t* v, operatorlib_strides_t v_strides,
+    const float* slopes, const int32_t* documents, const int32_t* prefixes,
+    operatorlib_half_t* output, operatorlib_strides_t output_strides, int batch, int q_heads,
+    int kv_heads, int sequence, int head_dim, float scale, int causal, int window, float softcap,
+    void* stream) {
+  const auto in = [](const operatorlib_half_t* p) { return reinterpret_cast<const _Float16*>(p); };
+  return masked_entry<_Float16>(
+      {in(q), in(k), in(v), reinterpret_cast<_Float16*>(output), of(q_strides), of(k_strides),
+       of(v_strides), of(output_strides), slopes, documents, prefixes, 0, q_heads, 1, sequence,
+       head_dim, causal != 0, window, {}},
+      batch, kv_heads, scale, softcap, stream);
+}
+
+extern "C" int operatorlib_masked_attention_f32(
+    const float* q, operatorlib_strides_t q_strides, const float* k,
+    operatorlib_strides_t k_strides, const float* v, operatorlib_strides_t v_strides,
+    const float* slopes, const int32_t* documents, const int32_t* prefixes, float* output,
+    operatorlib_strides_t output_strides, int batch, int q_heads, int kv_heads, int sequence,
+    int head_dim, float scale, int causal, int window, float softcap, void* stream) {
+  return masked_entry<float>({q, k, v, output, of(q_strides), of(k_strides), of(v_strides),
+                              of(output_strides), slopes, documents, prefixes, 0, q_heads, 1,
+                              sequence, head_dim, causal != 0, window, {}},
+                             batch, kv_heads, scale, softcap, stream);
+}

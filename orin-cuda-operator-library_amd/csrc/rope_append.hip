@@ -1,0 +1,251 @@
+// rope_append: rotates a step's queries and keys and stores its keys and
+// values in a paged cache (operatorlib/lm_c.h).
+//
+// Pair (a, b) of a head -> (a cos t - b sin t, b cos t + a sin t) with
+// t = position * frequency. The product is taken in 64 bits and reduced to a
+// fraction of a turn there: in 32 bits position 131072 times frequency 1
+// would leave an angle known to 2^-8 radians. cos and sin of the fraction
+// are taken in fp32 (an error of 2^-24 of a turn before, 2 ulp after), the
+// rotation in fp32, each output rounded to its type once.
+//
+// Every element is read once and written once or twice: bound by HBM. One
+// workgroup handles a token, or a share of its elements when there are few
+// tokens; 16-byte chunks, one rotation item being two chunks half a rotary
+// width apart (or one chunk of neighbouring pairs). The cos / sin table of
+// the token (at most a pair per thread and step) is computed once per
+// workgroup into LDS while the first chunks are in flight, and serves all of
+// its query and key heads.
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "common.hpp"
+#include "lm_validate.hpp"
+#include "operatorlib/lm_c.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTable = 512;  // pairs of the LDS table; wider rotations compute per item
+
+template <typename T, int E>
+struct Chunk {
+  typedef T type __attribute__((ext_vector_type(E)));
+};
+template <typename T>
+struct Chunk<T, 1> {
+  struct type {
+    T v;
+    __device__ T& operator[](int) { return v; }
+    __device__ const T& operator[](int) const { return v; }
+  };
+};
+
+template <typename T>
+struct RopeArgs {
+  const T* q;
+  const T* k;
+  const T* v;
+  std::int64_t q_stride, k_stride, v_stride;
+  const std::int32_t* positions;
+  const std::int32_t* axes;
+  const float* frequencies;
+  const std::int32_t* slots;
+  T* q_out;
+  T* k_out;
+  T* key_cache;
+  T* value_cache;
+  int tokens, position_rows, q_heads, kv_heads, head_dim, rotary_dim, cache_slots, page_size;
+  int parts;  // workgroups per token
+};
+
+// cos and sin of pair i's angle at token t.
+template <typename T>
+__device__ __forceinline__ float2 unit_of(const RopeArgs<T>& a, int t, int i) {
+  const int axis = a.axes == nullptr ? 0 : a.axes[i];
+  if (axis < 0 || axis >= a.position_rows) return make_float2(1.0f, 0.0f);
+  const double angle =
+      static_cast<double>(a.positions[static_cast<std::int64_t>(axis) * a.tokens + t]) *
+      static_cast<double>(a.frequencies[i]);
+  const double turns = angle * 0.15915494309189533577;  // 1 / (2 pi)
+  float s, c;
+  sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+  return make_float2(c, s);
+}
+
+// E: elements per access (a whole 16-byte chunk, or 1 on unaligned tensors).
+template <typename T, int E, bool kInterleaved>
+__global__ __launch_bounds__(kThreads) void rope_append_kernel(const RopeArgs<T> a) {
+  using C = typename Chunk<T, E>::type;
+  // Pair items: half-split, chunks (i, i + R / 2); interleaved, one chunk of
+  // E / 2 pairs (E = 1: the two elements of one pair).
+  constexpr int kPairs = kInterleaved ? (E == 1 ? 1 : E / 2) : E;  // pairs per item
+  constexpr bool kTwo = !kInterleaved || E == 1;                   // two accesses per item
+  __shared__ float2 table[kMaxTable];
+
+  const int t = static_cast<int>(blockIdx.x / a.parts);
+  const int part = static_cast<int>(blockIdx.x % a.parts);
+  const int pairs = a.rotary_dim / 2;
+  const bool in_table = pairs <= kMaxTable;
+  if (in_table) {
+    for (int i = threadIdx.x; i < pairs; i += kThreads) table[i] = unit_of(a, t, i);
+    __syncthreads();
+  }
+  const int slot = a.slots[t];
+  const bool stored = slot >= 0 && slot < a.cache_slots;
+  const int page = stored ? slot / a.page_size : 0;
+  const int row = stored ? slot - page * a.page_size : 0;
+  const std::int64_t d = a.head_dim;
+  const std::int64_t cache_row =
+      (static_cast<std::int64_t>(page) * a.kv_heads * a.page_size + row) * d;
+  const std::int64_t cache_head = a.page_size * d;
+
+  // Items: [pair items of q heads, of k heads][copied chunks past the rotary
+  // dims of q and k heads][chunks of v heads].
+  const int per_head = pairs / kPairs;
+  const int tail = (a.head_dim - a.rotary_dim) / E;
+  const int whole = a.head_dim / E;
+  const int qk = a.q_heads + a.kv_heads;
+  const int rotated = qk * per_head;
+  const int copied = rotated + qk * tail;
+  const int total = copied + a.kv_heads * whole;
+
+  for (int item = part * kThreads + threadIdx.x; item < total; item += a.parts * kThreads) {
+    if (item < copied) {
+      const bool rotate = item < rotated;
+      const int h = rotate ? item / per_head : (item - rotated) / tail;
+      const int j = rotate ? item - h * per_head : (item - rotated) - h * tail;
+      const bool is_q = h < a.q_heads;
+      const int hh = is_q ? h : h - a.q_heads;
+      const T* src = (is_q ? a.q + t * a.q_stride : a.k + t * a.k_stride) + hh * d;
+      T* out = is_q ? a.q_out + (static_cast<std::int64_t>(t) * a.q_heads + hh) * d
+                    : a.k_out + (static_cast<std::int64_t>(t) * a.kv_heads + hh) * d;
+      T* cache = a.key_cache + cache_row + hh * cache_head;
+      const bool to_out = is_q || a.k_out != nullptr;
+      const bool to_cache = !is_q && stored;
+      if (rotate) {
+        const int first = j * kPairs;  // pair
+        const int lo = kInterleaved ? 2 * first : first;
+        const int hi = kInterleaved ? lo + 1 : lo + pairs;
+        C x = *reinterpret_cast<const C*>(src + lo);
+        C y = x;
+        if constexpr (kTwo) y = *reinterpret_cast<const C*>(src + hi);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          const float2 u = in_table ? table[first + e] : unit_of(a, t, first + e);
+          if constexpr (kTwo) {
+            const float p = static_cast<float>(x[e]), q = static_cast<float>(y[e]);
+            x[e] = static_cast<T>(p * u.x - q * u.y);
+            y[e] = static_cast<T>(q * u.x + p * u.y);
+          } else {
+            const float p = static_cast<float>(x[2 * e]), q = static_cast<float>(x[2 * e + 1]);
+            x[2 * e] = static_cast<T>(p * u.x - q * u.y);
+            x[2 * e + 1] = static_cast<T>(q * u.x + p * u.y);
+          }
+        }
+        if (to_out) {
+          *reinterpret_cast<C*>(out + lo) = x;
+          if constexpr (kTwo) *reinterpret_cast<C*>(out + hi) = y;
+        }
+        if (to_cache) {
+          *reinterpret_cast<C*>(cache + lo) = x;
+          if constexpr (kTwo) *reinterpret_cast<C*>(cache + hi) = y;
+        }
+      } else {
+        const int at = a.rotary_dim + j * E;
+        const C x = *reinterpret_cast<const C*>(src + at);
+        if (to_out) *reinterpret_cast<C*>(out + at) = x;
+        if (to_cache) *reinterpret_cast<C*>(cache + at) = x;
+      }
+    } else if (stored) {
+      const int h = (item - copied) / whole;
+      const int at = ((item - copied) - h * whole) * E;
+      *reinterpret_cast<C*>(a.value_cache + cache_row + h * cache_head + at) =
+          *reinterpret_cast<const C*>(a.v + t * a.v_stride + h * d + at);
+    }
+  }
+}
+
+template <typename T, int E>
+hipError_t launch(RopeArgs<T> a, bool interleaved, hipStream_t stream) {
+  const int pairs = a.rotary_dim / 2;
+  const long long per_head =
+      interleaved && E > 1 ? pairs / (E / 2) : pairs / E;
+  const long long items =
+      (a.q_heads + a.kv_heads) * (per_head + (a.head_dim - a.rotary_dim) / E) +
+      static_cast<long long>(a.kv_heads) * (a.head_dim / E);
+  // Few tokens: a workgroup per 256 items, so that a step of few sequences
+  // spreads over the CUs; many tokens: one workgroup each.
+  long long parts = (items + kThreads - 1) / kThreads;
+  const long long spread = (1024 + a.tokens - 1) / a.tokens;
+  if (parts > spread) parts = spread;
+  if (parts * a.tokens > opl::kInt32Max) return hipErrorInvalidValue;
+  a.parts = static_cast<int>(parts);
+  const dim3 grid(static_cast<unsigned>(parts * a.tokens));
+  if (interleaved)
+    rope_append_kernel<T, E, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+  else
+    rope_append_kernel<T, E, false><<<grid, dim3(kThreads), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+int rope_entry(RopeArgs<T> a, int interleaved, int pages, void* stream_handle) {
+  const opl::RopeShape shape = {a.q_stride, a.k_stride,  a.v_stride,   a.position_rows, a.tokens,
+                                a.q_heads,  a.kv_heads,  a.head_dim,   a.rotary_dim,    pages,
+                                a.page_size};
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.slots == nullptr ||
+      a.q_out == nullptr || a.key_cache == nullptr || a.value_cache == nullptr ||
+      a.key_cache == a.value_cache || !opl::rope_shape_ok(shape))
+    return hipErrorInvalidValue;
+  if (a.rotary_dim > 0 && (a.positions == nullptr || a.frequencies == nullptr))
+    return hipErrorInvalidValue;
+  a.cache_slots = pages * a.page_size;
+  constexpr int E = 16 / sizeof(T);
+  const int unit = interleaved ? a.rotary_dim : a.rotary_dim / 2;
+  const bool chunks = a.head_dim % E == 0 && unit % E == 0 &&
+                      opl::aligned_rows(a.q, sizeof(T), a.q_stride) &&
+                      opl::aligned_rows(a.k, sizeof(T), a.k_stride) &&
+                      opl::aligned_rows(a.v, sizeof(T), a.v_stride) &&
+                      opl::aligned16(a.q_out) && opl::aligned16(a.k_out) &&
+                      opl::aligned16(a.key_cache) && opl::aligned16(a.value_cache);
+  const hipStream_t stream = static_cast<hipStream_t>(stream_handle);
+  return chunks ? launch<T, E>(a, interleaved != 0, stream)
+                : launch<T, 1>(a, interleaved != 0, stream);
+}
+
+}  // namespace
+
+extern "C" int operatorlib_lm_abi_version(void) { return OPERATORLIB_LM_ABI_VERSION; }
+
+extern "C" int operatorlib_rope_append_f16(
+    const operatorlib_half_t* q, int64_t q_token_stride, const operatorlib_half_t* k,
+    int64_t k_token_stride, const operatorlib_half_t* v, int64_t v_token_stride,
+    const int32_t* positions, int position_rows, const int32_t* axes, const float* frequencies,
+    const int32_t* slots, operatorlib_half_t* q_out, operatorlib_half_t* k_out,
+    operatorlib_half_t* key_cache, operatorlib_half_t* value_cache, int tokens, int q_heads,
+    int kv_heads, int head_dim, int rotary_dim, int interleaved, int pages, int page_size,
+    void* stream) {
+  const auto in = [](const operatorlib_half_t* p) { return reinterpret_cast<const _Float16*>(p); };
+  const auto out = [](operatorlib_half_t* p) { return reinterpret_cast<_Float16*>(p); };
+  return rope_entry<_Float16>(
+      {in(q), in(k), in(v), q_token_stride, k_token_stride, v_token_stride, positions, axes,
+       frequencies, slots, out(q_out), out(k_out), out(key_cache), out(value_cache), tokens,
+       position_rows, q_heads, kv_heads, head_dim, rotary_dim, 0, page_size, 1},
+      interleaved, pages, stream);
+}
+
+extern "C" int operatorlib_rope_append_f32(
+    const float* q, int64_t q_token_stride, const float* k, int64_t k_token_stride, const float* v,
+    int64_t v_token_stride, const int32_t* positions, int position_rows, const int32_t* axes,
+    const float* frequencies, const int32_t* slots, float* q_out, float* k_out, float* key_cache,
+    float* value_cache, int tokens, int q_heads, int kv_heads, int head_dim, int rotary_dim,
+    int interleaved, int pages, int page_size, void* stream) {
+  return rope_entry<float>(
+      {q, k, v, q_token_stride, k_token_stride, v_token_stride, positions, axes, frequencies,
+       slots, q_out, k_out, key_cache, value_cache, tokens, position_rows, q_heads, kv_heads,
+       head_dim, rotary_dim, 0, page_size, 1},
+      interleaved, pages, stream);
+}

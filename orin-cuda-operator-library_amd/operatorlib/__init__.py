@@ -1,8 +1,9 @@
 """operatorlib for MI355X — Python entry points.
 
 * ``load_operatorlib()`` registers ``torch.ops.operatorlib.{reduce_sum,
-  softmax, transpose, rmsnorm, gemm, attention}`` from the in-tree
-  extension. Like the reference's ``python/load_extension.py:17-36``, which
+  softmax, transpose, rmsnorm, gemm, attention}`` and the language-model
+  operators ``{rope_append, paged_attention, masked_attention}`` from the
+  in-tree extension. Like the reference's ``python/load_extension.py:17-36``, which
   compiles its CUDA sources on first use, it builds the HIP library and the
   binding with hipcc for gfx950 when they are not built yet
   (``OPERATORLIB_NO_BUILD=1`` turns that off); a build that exists is loaded
@@ -11,6 +12,8 @@
   C ABI of ``include/operatorlib/operatorlib_c.h`` typed, for callers that
   want the library without the torch layer. It builds on first use in the
   same way.
+* ``lm_clib()`` does the same for ``liboperatorlib_lm.so`` and the C ABI of
+  ``include/operatorlib/lm_c.h``.
 
 Both raise if the native library is missing and cannot be built: there is
 no fallback implementation.
@@ -26,10 +29,12 @@ from . import _build
 
 LIB_DIR = _build.LIB_DIR
 LIBRARY_PATH = _build.LIBRARY
+LM_LIBRARY_PATH = _build.LM_LIBRARY
 TORCH_EXT_PATH = _build.TORCH_EXT
 
-__all__ = ["build", "load_operatorlib", "clib", "LIBRARY_PATH", "TORCH_EXT_PATH",
-           "C_SYMBOLS", "HIP_SUCCESS", "HIP_ERROR_INVALID_VALUE"]
+__all__ = ["build", "load_operatorlib", "clib", "lm_clib", "LIBRARY_PATH", "LM_LIBRARY_PATH",
+           "TORCH_EXT_PATH", "C_SYMBOLS", "LM_C_SYMBOLS", "Strides", "HIP_SUCCESS",
+           "HIP_ERROR_INVALID_VALUE"]
 
 HIP_SUCCESS = 0
 HIP_ERROR_INVALID_VALUE = 1
@@ -105,7 +110,30 @@ C_SYMBOLS = {
                                                 _c.c_void_p]),
 }
 
+
+class Strides(_c.Structure):
+    """operatorlib_strides_t: element strides of [batch, heads, sequence, head_dim]."""
+    _fields_ = [("batch", _c.c_int64), ("head", _c.c_int64), ("token", _c.c_int64)]
+
+
+_p, _i, _l, _f = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float
+_ROPE = [_p, _l, _p, _l, _p, _l, _p, _i, *[_p] * 7, *[_i] * 8, _p]
+_PAGED = [_p, _l, _p, _p, _p, _l, *[_p] * 3, *[_i] * 7, _f, _i, _f]
+_MASKED = [_p, Strides, _p, Strides, _p, Strides, _p, _p, _p, _p, Strides, *[_i] * 5, _f, _i, _i,
+           _f, _p]
+# name -> (restype, argtypes); mirrors include/operatorlib/lm_c.h
+LM_C_SYMBOLS = {"operatorlib_lm_abi_version": (_i, [])}
+for _t in ("f16", "f32"):
+    LM_C_SYMBOLS |= {
+        f"operatorlib_rope_append_{_t}": (_i, _ROPE),
+        f"operatorlib_paged_attention_{_t}_workspace_size": (_c.c_size_t, [_i] * 6),
+        f"operatorlib_paged_attention_{_t}": (_i, [*_PAGED, _p]),
+        f"operatorlib_paged_attention_{_t}_ws": (_i, [*_PAGED, _p, _c.c_size_t, _p]),
+        f"operatorlib_masked_attention_{_t}": (_i, _MASKED),
+    }
+
 _clib = None
+_lm_clib = None
 _torch_loaded = False
 
 
@@ -146,13 +174,27 @@ def clib() -> ctypes.CDLL:
             import torch  # noqa: F401
         except ImportError:
             pass
-        lib = ctypes.CDLL(str(LIBRARY_PATH), mode=ctypes.RTLD_GLOBAL)
-        for name, (restype, argtypes) in C_SYMBOLS.items():
-            fn = getattr(lib, name)
-            fn.restype = restype
-            fn.argtypes = argtypes
-        _clib = lib
+        _clib = _typed(LIBRARY_PATH, C_SYMBOLS)
     return _clib
+
+
+def lm_clib() -> ctypes.CDLL:
+    """Load ``liboperatorlib_lm.so`` and type its C ABI."""
+    global _lm_clib
+    if _lm_clib is None:
+        _require(LM_LIBRARY_PATH, torch_binding=False)
+        clib()  # liboperatorlib.so, which it links
+        _lm_clib = _typed(LM_LIBRARY_PATH, LM_C_SYMBOLS)
+    return _lm_clib
+
+
+def _typed(path: Path, symbols: dict) -> ctypes.CDLL:
+    lib = ctypes.CDLL(str(path), mode=ctypes.RTLD_GLOBAL)
+    for name, (restype, argtypes) in symbols.items():
+        fn = getattr(lib, name)
+        fn.restype = restype
+        fn.argtypes = argtypes
+    return lib
 
 
 def load_operatorlib(verbose: bool = False) -> None:
@@ -162,7 +204,7 @@ def load_operatorlib(verbose: bool = False) -> None:
         return
     import torch
     _require(TORCH_EXT_PATH, torch_binding=True)
-    clib()  # the extension links liboperatorlib.so; load it first, same runtime
+    lm_clib()  # the extension links both libraries; load them first, same runtime
     torch.ops.load_library(str(TORCH_EXT_PATH))
     if verbose:
         print(f"loaded {TORCH_EXT_PATH}")

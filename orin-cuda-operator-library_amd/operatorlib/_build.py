@@ -3,6 +3,9 @@
 Outputs (all under ``orin-cuda-operator-library_amd/operatorlib/lib``):
   * ``liboperatorlib.so``      — HIP kernels + the C ABI
                                  (include/operatorlib/operatorlib_c.h)
+  * ``liboperatorlib_lm.so``   — the language-model operators' kernels + C ABI
+                                 (include/operatorlib/lm_c.h); links
+                                 liboperatorlib.so
   * ``operatorlib_run``        — standalone key=value runner (runner/)
   * ``_operatorlib_torch.so``  — ``torch.ops.operatorlib.*`` registrations
                                  (same schema as the reference's
@@ -49,7 +52,10 @@ LIB_SOURCES = [
     "gemm.hip", "attention.hip", "scratch.hip", "capi.cpp",
 ]
 
+LM_SOURCES = ["rope_append.hip", "paged_attention.hip", "masked_attention.hip"]
+
 LIBRARY = LIB_DIR / "liboperatorlib.so"
+LM_LIBRARY = LIB_DIR / "liboperatorlib_lm.so"
 TORCH_EXT = LIB_DIR / "_operatorlib_torch.so"
 
 
@@ -78,15 +84,20 @@ def _jobs() -> int:
 
 
 def build_library(verbose: bool = False) -> Path:
+    """liboperatorlib.so and, linked against it, liboperatorlib_lm.so."""
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     with ThreadPoolExecutor(_jobs()) as pool:
         objs = list(pool.map(
             lambda s: _compile(CSRC / s, OBJ_DIR / (s + ".o"), [], verbose),
-            LIB_SOURCES))
+            LIB_SOURCES + LM_SOURCES))
+    link = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}"]
     tmp = LIBRARY.with_suffix(".so.tmp")
-    _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}",
-          *[str(o) for o in objs], "-o", str(tmp)], verbose)
+    _run([*link, *[str(o) for o in objs[:len(LIB_SOURCES)]], "-o", str(tmp)], verbose)
     os.replace(tmp, LIBRARY)
+    tmp = LM_LIBRARY.with_suffix(".so.tmp")
+    _run([*link, *[str(o) for o in objs[len(LIB_SOURCES):]], f"-L{LIB_DIR}", "-loperatorlib",
+          "-Wl,-rpath,$ORIGIN", "-o", str(tmp)], verbose)
+    os.replace(tmp, LM_LIBRARY)
     return LIBRARY
 
 
@@ -106,11 +117,13 @@ def _torch_flags() -> tuple[list[str], list[str]]:
 
 def build_torch_binding(verbose: bool = False) -> Path:
     cflags, ldflags = _torch_flags()
-    obj = _compile(CSRC / "torch_binding.cpp", OBJ_DIR / "torch_binding.cpp.o",
-                   cflags, verbose)
+    with ThreadPoolExecutor(_jobs()) as pool:
+        objs = list(pool.map(
+            lambda s: _compile(CSRC / s, OBJ_DIR / (s + ".o"), cflags, verbose),
+            ["torch_binding.cpp", "torch_binding_lm.cpp"]))
     tmp = TORCH_EXT.with_suffix(".so.tmp")
-    _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", str(obj),
-          f"-L{LIB_DIR}", "-loperatorlib", "-Wl,-rpath,$ORIGIN", *ldflags,
+    _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *[str(o) for o in objs],
+          f"-L{LIB_DIR}", "-loperatorlib_lm", "-loperatorlib", "-Wl,-rpath,$ORIGIN", *ldflags,
           "-o", str(tmp)], verbose)
     os.replace(tmp, TORCH_EXT)
     return TORCH_EXT
