@@ -19,11 +19,12 @@
 //     whether all of them and all rows are one document; unmarked tiles are
 //     skipped, tiles of one document inside the bounds need no mask.
 //   * A wavefront applies the mask only in tiles that some of its rows see in
-//     part.
+//     part: a branch around the mask alone. (One loop body for both kinds of
+//     tile; two bodies made the compiler keep O twice and spill 139 registers.)
 //   * A hidden key's probability is 0, but 0 x infinity is NaN: if a block's O
-//     ends with a NaN, the block runs again and keeps, in the tiles that are
-//     seen in part, non-finite values out of the matrix product; they are
-//     added to the rows that see them. Blocks without a NaN pay one test.
+//     ends with a NaN, the block runs again with the non-finite values of V
+//     taken for zeros, and then adds them to the rows that see their keys.
+//     Blocks without a NaN pay one test.
 
 #include <hip/hip_runtime.h>
 
@@ -212,8 +213,15 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     }
     row_lo[qc] = low(i);
     row_span[qc] = high(i) - row_lo[qc];
-    row_doc[qc] = docs != nullptr ? docs[i] : 0;
+    row_doc[qc] = 0;  // without documents every key's id is read as 0
+    if (docs != nullptr) row_doc[qc] = docs[i] >= 0 ? docs[i] : -2;  // no key's id
   }
+  // Whether the lane's row of block qc sees a key whose document is id (-1: none).
+  auto sees = [&](int qc, int key, int id) -> bool {
+    const bool near = static_cast<unsigned>(key - row_lo[qc]) <= static_cast<unsigned>(row_span[qc]);
+    return ((near) | (key < prefix)) & (id == row_doc[qc]);
+  };
+  const float row_at = static_cast<float>(wave_row0 + col);
   const float slope = kRules && a.slopes != nullptr ? a.slopes[head] * opl::kLog2e : 0.0f;
 
   // ---- copies of a tile: byte offset of the lane's chunks, swizzled
@@ -272,8 +280,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   const float scale = kRules ? 1.0f : a.rules.scale;
   const float inv_scale = 1.0f / scale;
 
-  auto run = [&](auto exact_tag) {
-    constexpr bool kExact = decltype(exact_tag)::value;
+  for (bool exact = false;; exact = true) {
 #pragma unroll
     for (int qc = 0; qc < 2; ++qc) {
 #pragma unroll
@@ -284,20 +291,9 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       move_above[qc] = -INFINITY;
     }
 
-    auto body = [&](const unsigned char* cur, int key0, auto masked_tag) {
-      constexpr bool kMasked = decltype(masked_tag)::value;
+    auto body = [&](const unsigned char* cur, int key0, bool whole) {
       constexpr int kHalves = kTileKeys / 32;
       floatx4 s[kHalves][2][2];  // [32 keys][16 keys][qc]
-      int ids[kHalves][2][4];
-      if (kMasked && docs != nullptr) {
-#pragma unroll
-        for (int j = 0; j < kHalves; ++j)
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              ids[j][kb][e] = docs[min(key0 + 32 * j + 16 * kb + 4 * quad + e, S - 1)];
-      }
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int j = 0; j < kHalves; ++j) {
@@ -338,9 +334,52 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         }
       }
       __builtin_amdgcn_s_setprio(0);
+      if constexpr (kRules) {  // into log2 units: capped or scaled, then biased
+        auto each = [&](auto rule) {
+#pragma unroll
+          for (int j = 0; j < kHalves; ++j)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  s[j][kb][qc][e] = rule(s[j][kb][qc][e], qc, 32 * j + 16 * kb + e);
+        };
+        if (a.rules.cap != 0.0f)
+          each([&](float x, int, int) { return a.rules.template capped<!kHalf>(x); });
+        else
+          each([&](float x, int, int) { return x * a.rules.scale; });
+        if (a.slopes != nullptr) {
+          // distances are exact: positions are below 2^20
+          const float first = static_cast<float>(key0 + 4 * quad);
+          const float from[2] = {row_at - first, row_at + 16.0f - first};
+          each([&](float x, int qc, int key) {
+            return fmaf(-slope, fabsf(from[qc] - static_cast<float>(key)), x);
+          });
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < kHalves; ++j)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const int key = key0 + 32 * j + 16 * kb + 4 * quad;
+            int ids[4] = {};
+            if (docs != nullptr) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) ids[e] = max(docs[min(key + e, S - 1)], -1);
+            }
+#pragma unroll
+            for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[j][kb][qc][e] = sees(qc, key + e, ids[e]) ? s[j][kb][qc][e] : -INFINITY;
+          }
+      }
       float raw[2];
 #pragma unroll
-      for (int qc = 0; qc < 2; ++qc) raw[qc] = -INFINITY;
+      for (int qc = 0; qc < 2; ++qc) raw[qc] = s[0][0][qc][0];
 #pragma unroll
       for (int j = 0; j < kHalves; ++j)
 #pragma unroll
@@ -348,23 +387,8 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
           for (int qc = 0; qc < 2; ++qc)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = key0 + 32 * j + 16 * kb + 4 * quad + e;
-              float x = s[j][kb][qc][e];
-              if constexpr (kRules) {
-                x = a.rules.template log2_score<!kHalf>(x);
-                if (a.slopes != nullptr)
-                  x -= slope * fabsf(static_cast<float>(wave_row0 + 16 * qc + col - key));
-              }
-              if constexpr (kMasked) {
-                bool seen = static_cast<unsigned>(key - row_lo[qc]) <= static_cast<unsigned>(row_span[qc]) ||
-                            key < prefix;
-                if (docs != nullptr) seen = seen && ids[j][kb][e] == row_doc[qc] && row_doc[qc] >= 0;
-                if (!seen) x = -INFINITY;
-              }
-              s[j][kb][qc][e] = x;
-              raw[qc] = __builtin_elementwise_maximum(raw[qc], x);
-            }
+            for (int e = 0; e < 4; ++e)
+              raw[qc] = __builtin_elementwise_maximum(raw[qc], s[j][kb][qc][e]);
       if (__builtin_amdgcn_ballot_w64(raw[0] > move_above[0] || raw[1] > move_above[1]) != 0) {
 #pragma unroll
         for (int qc = 0; qc < 2; ++qc) {
@@ -378,21 +402,6 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
           for (int db = 0; db < L::kDBlocks; ++db) o[qc][db] *= alpha;
         }
-      }
-      // Exact pass, tile seen in part: are there non-finite values in it?
-      bool poisoned = false;
-      if constexpr (kExact && kMasked) {
-        bool bad = false;
-        for (int i = lane; i < L::kTile / 4; i += opl::kWaveSize) {
-          if constexpr (kHalf) {
-            const unsigned u = *reinterpret_cast<const unsigned*>(cur + L::kTile + 4 * i);
-            bad |= (((u & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
-          } else {
-            const unsigned u = *reinterpret_cast<const unsigned*>(cur + L::kTile + 4 * i);
-            bad |= (u & 0x7f800000u) == 0x7f800000u;
-          }
-        }
-        poisoned = __builtin_amdgcn_ballot_w64(bad) != 0;
       }
 #pragma unroll
       for (int j = 0; j < kHalves; ++j) {
@@ -417,13 +426,6 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
             for (int e = 0; e < 4; ++e) {
               f[e] = lo4[e];
               f[4 + e] = hi4[e];
-            }
-            if constexpr (kExact && kMasked) {
-              if (poisoned) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (!(fabsf(static_cast<float>(f[e])) < INFINITY)) f[e] = static_cast<_Float16>(0.0f);
-              }
             }
 #pragma unroll
             for (int qc = 0; qc < 2; ++qc)
@@ -452,9 +454,6 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
               for (int db = 0; db < L::kDBlocks; ++db) {
                 f[db] = *reinterpret_cast<const float*>(cur + v_base[db] + rows + (16 * kb + e) * L::kRowBytes);
-                if constexpr (kExact && kMasked) {
-                  if (poisoned && !(fabsf(f[db]) < INFINITY)) f[db] = 0.0f;
-                }
               }
 #pragma unroll
               for (int db = 0; db < L::kDBlocks; ++db)
@@ -462,30 +461,6 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
                 for (int qc = 0; qc < 2; ++qc)
                   o[qc][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[db], p[qc][kb][e], o[qc][db], 0, 0, 0);
             }
-        }
-      }
-      // The non-finite values go to the rows that see their keys.
-      if constexpr (kExact && kMasked) {
-        if (poisoned) {
-          for (int r = 0; r < kTileKeys && key0 + r < S; ++r) {
-            const int key = key0 + r;
-            const int id = docs != nullptr ? docs[key] : 0;
-#pragma unroll
-            for (int qc = 0; qc < 2; ++qc) {
-              bool seen = static_cast<unsigned>(key - row_lo[qc]) <= static_cast<unsigned>(row_span[qc]) || key < prefix;
-              if (docs != nullptr) seen = seen && id == row_doc[qc] && row_doc[qc] >= 0;
-#pragma unroll
-              for (int db = 0; db < L::kDBlocks; ++db)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int d = 16 * db + 4 * quad + e;
-                  const float x = static_cast<float>(*reinterpret_cast<const T*>(
-                      cur + L::kTile + r * L::kRowBytes +
-                      (((d / L::kElems) ^ L::swizzle_v(r)) * 16) + (d % L::kElems) * L::kSize));
-                  if (seen && !(fabsf(x) < INFINITY)) o[qc][db][e] += x;
-                }
-            }
-          }
         }
       }
     };
@@ -496,10 +471,23 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       for (int g = 0; g < kGroups; ++g) t = visit(t + 1);
       return t;
     };
+    // Exact pass: non-finite values of the arrived tile become zeros.
+    auto drop_non_finite = [&](unsigned char* cur) {  // (by the group's wavefronts)
+      const int first = (kW == 1 ? 0 : wave) * opl::kWaveSize + lane;
+      for (int i = first; i < L::kTile / L::kSize; i += kW * opl::kWaveSize) {
+        T* const x = reinterpret_cast<T*>(cur + L::kTile) + i;
+        if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = T(0);
+      }
+    };
     auto tile = [&](const unsigned char* cur, unsigned char* nxt, int t) {
       const int after = t < end_tile ? advance(t) : end_tile;
       if (after < end_tile) issue(nxt, after * kTileKeys);
       __builtin_amdgcn_sched_barrier(0);
+      if (exact) {
+        if (t < end_tile) drop_non_finite(const_cast<unsigned char*>(cur));
+        __builtin_amdgcn_s_waitcnt(0);
+        if constexpr (kW > 1) __syncthreads();  // (all groups, also those without a tile)
+      }
       const int key0 = t * kTileKeys;
       const int key1 = key0 + kTileKeys - 1;
       const int row0 = wave_row0, row1 = min(wave_row0 + kRowsPerWave, S) - 1;
@@ -510,10 +498,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
           const int bit = key0 / 64;
           whole = whole && ((single[bit / 32] >> (bit % 32)) & 1) != 0;
         }
-        if (__builtin_amdgcn_readfirstlane(whole))
-          body(cur, key0, std::false_type{});
-        else
-          body(cur, key0, std::true_type{});
+        body(cur, key0, whole);
       }
       __builtin_amdgcn_s_waitcnt(0);
       if constexpr (kW == 1) {
@@ -548,10 +533,9 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       }
     }
     __syncthreads();  // every stage is free
-  };
-
-  run(std::false_type{});
-  {
+    if (exact) break;
+    // A NaN in O: a non-finite value was multiplied by a hidden key's 0, or is
+    // seen.
     bool bad = false;
 #pragma unroll
     for (int qc = 0; qc < 2; ++qc)
@@ -563,9 +547,8 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     __syncthreads();
     if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) again = 1;
     __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(again)) run(std::true_type{});
+    if (__builtin_amdgcn_readfirstlane(again) == 0) break;
   }
-
   // ---- join the groups, normalise, store whole rows through LDS
   float row_sum[2], coef[2];
 #pragma unroll
@@ -601,6 +584,34 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
     for (int qc = 0; qc < 2; ++qc) coef[qc] = inverse(row_sum[qc]);
   }
+#pragma unroll
+  for (int qc = 0; qc < 2; ++qc)
+#pragma unroll
+    for (int db = 0; db < L::kDBlocks; ++db) o[qc][db] *= coef[qc];
+  if (__builtin_amdgcn_readfirstlane(again) != 0) {
+    // The non-finite values go to the rows that see their keys, after the
+    // weights (infinity times a weight of 0 is NaN); one group adds them, as
+    // the groups' O are summed.
+    typedef T Four __attribute__((ext_vector_type(4)));
+    for (int t = group == 0 ? visit(0) : end_tile; t < end_tile; t = visit(t + 1)) {
+      for (int key = t * kTileKeys; key < min((t + 1) * kTileKeys, S); ++key) {
+        const int id = docs != nullptr ? max(docs[key], -1) : 0;
+        const T* const row = vh + static_cast<std::int64_t>(key) * a.vs.token;
+#pragma unroll
+        for (int db = 0; db < L::kDBlocks; ++db) {
+          const int d = 16 * db + 4 * quad;
+          const Four x = *reinterpret_cast<const Four*>(row + (d < dm ? d : 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = static_cast<float>(x[e]);
+            if (fabsf(y) < INFINITY) continue;
+#pragma unroll
+            for (int qc = 0; qc < 2; ++qc) o[qc][db][e] += sees(qc, key, id) ? y : 0.0f;
+          }
+        }
+      }
+    }
+  }
   constexpr int kBlockBytes = kRowsPerWave * D * 4;
   constexpr int kPerArray = kArray / kBlockBytes;
   static_assert(kPerArray >= 1 && kGroups * kW <= 2 * kPerArray, "blocks fit the stage arrays");
@@ -616,7 +627,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
       for (int db = 0; db < L::kDBlocks; ++db) {
         const int r = 16 * qc + col;
-        to[r * kQuads + ((4 * db + quad) ^ (r % kQuads))] = o[qc][db] * coef[qc];
+        to[r * kQuads + ((4 * db + quad) ^ (r % kQuads))] = o[qc][db];
       }
   }
   __syncthreads();

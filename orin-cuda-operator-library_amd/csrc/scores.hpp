@@ -35,9 +35,13 @@ struct ScoreRules {
   }
 
   template <bool kPrecise>
+  __device__ __forceinline__ float capped(float dot) const {
+    return cap * tanh_of<kPrecise>(dot * scale);
+  }
+
+  template <bool kPrecise>
   __device__ __forceinline__ float log2_score(float dot) const {
-    const float y = dot * scale;
-    return cap != 0.0f ? cap * tanh_of<kPrecise>(y) : y;
+    return cap != 0.0f ? capped<kPrecise>(dot) : dot * scale;
   }
 };
 
