@@ -180,6 +180,15 @@ __device__ __forceinline__ void buffer_copy16_lds(const void* base, unsigned byt
       (__attribute__((address_space(3))) void*)dst, 16, voffset, 0, 0, Aux);
 }
 
+// The same for 4 bytes per lane, into LDS at dst + 4 * lane.
+__device__ __forceinline__ void buffer_copy4_lds(const void* base, unsigned bytes, void* dst,
+                                                 int voffset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0),
+                                        bytes, kBufferFlags),
+      (__attribute__((address_space(3))) void*)dst, 4, voffset, 0, 0, 0);
+}
+
 // max / sum of v over lanes l and l ^ 32 (the two halves of a wavefront),
 // the same value in both lanes. v_permlane32_swap exchanges the halves
 // register to register, where __shfl_xor(v, 32) is an LDS round trip

@@ -15,9 +15,11 @@
 //     lo(i) <= j <= hi(i): two compares. lo and hi come from causal and window.
 //   * A query block visits the key tiles of the prefix and of
 //     [lo(first row), hi(last row)] only. With documents it first marks, per
-//     64 keys, whether any of them is in the block's span of documents, and
-//     whether all of them and all rows are one document; unmarked tiles are
-//     skipped, tiles of one document inside the bounds need no mask.
+//     wavefront and 64 keys, whether their span of documents meets that of the
+//     wavefront's rows, and whether all of them and all rows are one
+//     document: tiles that no wavefront marks are not copied, a wavefront skips
+//     those it has not marked, and tiles of one document inside the bounds need
+//     no mask. The tiles' ids are copied to LDS with the tiles.
 //   * A wavefront applies the mask only in tiles that some of its rows see in
 //     part: a branch around the mask alone. (One loop body for both kinds of
 //     tile; two bodies made the compiler keep O twice and spill 139 registers.)
@@ -53,7 +55,10 @@ constexpr int kRowsPerWave = 32;
 constexpr float kLazyLog2 = 8.0f;
 // Workgroup slots of an XCD that a causal launch balances (attention.hip).
 constexpr int kCausalGroupSlots = 64;
-constexpr int kMarkWords = opl::kMaxMaskedSequence / 64 / 32;  // a bit per 64 keys
+// Marks: a bit per 64 keys, up to 2^18 keys; tiles behind those are visited and
+// masked whatever their documents.
+constexpr int kMarkWords = 128;
+constexpr int kIdBytes = 256;  // ids of a tile's keys in LDS, as one wavefront copies them
 
 template <typename T>
 struct MaskedArgs {
@@ -76,11 +81,12 @@ constexpr int kMinWavesPerSimd =
 // kW wavefronts of 32 query rows share the tiles of a group; kGroups groups
 // (small grids) take every kGroups-th tile of the same rows and join at the
 // end. kRules: scores are capped or biased (else they are only scaled).
-template <typename T, int D, int kGroups, int kW, int kTileKeys, bool kRules>
+// D: the LDS rows' dims; Dc: those computed (head dims of 65 to 96 take 96 of 128).
+template <typename T, int D, int Dc, int kGroups, int kW, int kTileKeys, bool kRules>
 __global__ __launch_bounds__(kW * opl::kWaveSize * kGroups)
 __attribute__((amdgpu_waves_per_eu(kMinWavesPerSimd<T, D, kGroups, kW, kTileKeys>, 2)))
 void masked_attention_kernel(const MaskedArgs<T> a) {
-  using L = opl::Layout<T, D, kTileKeys>;
+  using L = opl::Layout<T, D, kTileKeys, Dc>;
   constexpr bool kHalf = L::kSize == 2;
   using Frag = typename std::conditional<kHalf, half8, floatx4>::type;
   constexpr int kRows = kW * kRowsPerWave;
@@ -89,8 +95,12 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   constexpr int kArray = kGroups * L::kStage;
   __shared__ __attribute__((aligned(1024))) unsigned char stage0[kArray];
   __shared__ __attribute__((aligned(1024))) unsigned char stage1[kArray];
-  __shared__ unsigned marked[kMarkWords];  // some key of the 64 may be visible
-  __shared__ unsigned single[kMarkWords];  // all rows and all 64 keys are one document
+  __shared__ __attribute__((aligned(16))) int ids0[kGroups * kIdBytes / 4];
+  __shared__ __attribute__((aligned(16))) int ids1[kGroups * kIdBytes / 4];
+  __shared__ unsigned marked[kMarkWords];     // some wavefront's bit is set
+  __shared__ unsigned some[kW][kMarkWords];   // the documents of the 64 keys and its rows may meet
+  __shared__ unsigned single[kW][kMarkWords]; // its rows and the 64 keys are one document
+  __shared__ int span[kW][3];                 // least and greatest document of its rows, 1 if it has one
   __shared__ int again;
 
   // ---- which rows of which head: XCD x takes a contiguous range of the work,
@@ -123,6 +133,8 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   const int group = kGroups == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / opl::kWaveSize / kW);
   unsigned char* const st0 = stage0 + group * L::kStage;
   unsigned char* const st1 = stage1 + group * L::kStage;
+  int* const id0 = ids0 + group * (kIdBytes / 4);
+  int* const id1 = ids1 + group * (kIdBytes / 4);
   const int col = lane % 16;
   const int quad = lane / 16;
   const int wave_row0 = q0 + wave * kRowsPerWave;
@@ -147,38 +159,71 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   const int from_tile = low(q0) / kTileKeys;
   const int end_tile = max(prefix_tiles, high(last_row) / kTileKeys + 1);
   if (docs != nullptr) {
-    // The block's documents: the least and greatest id of its rows.
-    int least = 0x7fffffff, most = -1;
-    bool all = true;
-    for (int i = q0 + lane; i <= last_row; i += opl::kWaveSize) {
-      const int id = docs[i];
-      if (id >= 0) {
-        least = min(least, id);
-        most = max(most, id);
-      } else {
-        all = false;
-      }
-    }
+    // Lane l of a wavefront takes the 64 keys of chunk c0 + l: their least and
+    // greatest id. (A ballot per chunk, one key per lane, took 3.7 us of each
+    // workgroup at 8000 keys; a chunk per 16 lanes was no faster than this.)
+    struct Ids {
+      unsigned least_id;  // of the ids >= 0 (a negative one is a large unsigned)
+      int most_id, any_id;
+    };
+    auto ids_of = [&](int chunk) {
+      typedef int Four __attribute__((ext_vector_type(4), aligned(4)));
+      Ids r = {0xffffffffu, -1, 0x7fffffff};
+      auto take = [&](int id) {
+        r.least_id = min(r.least_id, static_cast<unsigned>(id));
+        r.most_id = max(r.most_id, id);
+        r.any_id = min(r.any_id, id);
+      };
+      const int first = chunk * 64;
+      if (first + 64 <= S) {
 #pragma unroll
-    for (int step = 1; step < opl::kWaveSize; step *= 2) {
-      least = min(least, __shfl_xor(least, step));
-      most = max(most, __shfl_xor(most, step));
+        for (int i = 0; i < 16; ++i) {
+          const Four id = *reinterpret_cast<const Four*>(docs + first + 4 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) take(id[e]);
+        }
+      } else {
+        for (int key = first; key < first + 64; ++key) take(key < S ? docs[key] : -1);
+      }
+      return r;
+    };
+    // Each wavefront of rows: the least and greatest id, by 32 of its lanes.
+    const int i = wave_row0 + lane % kRowsPerWave;
+    const int id = docs[min(i, S - 1)];
+    // The first step's keys are read before the rows' ids are awaited.
+    const int chunks = min((end_tile * kTileKeys + 63) / 64, kMarkWords * 32);
+    int c0 = threadIdx.x / opl::kWaveSize * 64;
+    Ids keys = ids_of(min(c0 + lane, chunks - 1));
+    int least_row = i < S && id >= 0 ? id : 0x7fffffff, most_row = i < S ? max(id, -1) : -1;
+#pragma unroll
+    for (int step = 1; step < kRowsPerWave; step *= 2) {
+      least_row = min(least_row, __shfl_xor(least_row, step));
+      most_row = max(most_row, __shfl_xor(most_row, step));
     }
-    const bool one = __builtin_amdgcn_ballot_w64(!all) == 0 && least == most;
-    const int chunks = (end_tile * kTileKeys + 63) / 64;
-    for (int word = threadIdx.x / opl::kWaveSize; word * 32 < chunks; word += kThreads / opl::kWaveSize) {
-      unsigned some = 0, same = 0;
-#pragma unroll 8
-      for (int bit = 0; bit < 32; ++bit) {
-        const int key = (word * 32 + bit) * 64 + lane;
-        const int id = key < S ? docs[key] : -1;
-        if (__builtin_amdgcn_ballot_w64(id >= least && id <= most) != 0) some |= 1u << bit;
-        if (one && __builtin_amdgcn_ballot_w64(id != least) == 0) same |= 1u << bit;
+    const bool padded = __builtin_amdgcn_ballot_w64(i < S && id < 0) != 0;
+    if (group == 0 && lane == 0) {
+      span[wave][0] = least_row;
+      span[wave][1] = most_row;
+      span[wave][2] = !padded && least_row == most_row;
+    }
+    __syncthreads();
+    for (; c0 < chunks; c0 += kThreads) {
+      std::uint64_t any = 0;
+#pragma unroll
+      for (int r = 0; r < kW; ++r) {
+        const int least = span[r][0], most = span[r][1];
+        const std::uint64_t within = __builtin_amdgcn_ballot_w64(
+            (most >= 0) & (keys.least_id <= static_cast<unsigned>(most)) & (keys.most_id >= least));
+        const std::uint64_t same = __builtin_amdgcn_ballot_w64(
+            (span[r][2] != 0) & (keys.any_id == least) & (keys.most_id == least));
+        any |= within;
+        if (lane < 2) {
+          some[r][c0 / 32 + lane] = static_cast<unsigned>(within >> (32 * lane));
+          single[r][c0 / 32 + lane] = static_cast<unsigned>(same >> (32 * lane));
+        }
       }
-      if (lane == 0) {
-        marked[word] = some;
-        single[word] = same;
-      }
+      if (lane < 2) marked[c0 / 32 + lane] = static_cast<unsigned>(any >> (32 * lane));
+      if (c0 + kThreads < chunks) keys = ids_of(min(c0 + kThreads + lane, chunks - 1));
     }
     __syncthreads();
   }
@@ -188,6 +233,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     if (docs != nullptr) {
       while (t < end_tile) {
         const int bit = t * kTileKeys / 64;
+        if (bit >= kMarkWords * 32) break;
         const unsigned rest = __builtin_amdgcn_readfirstlane(marked[bit / 32]) >> (bit % 32);
         if (rest & 1) break;
         // the next marked 64 keys of this word, or the next word
@@ -240,7 +286,11 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   const unsigned k_bytes = static_cast<unsigned>((S - 1) * a.ks.token + dm) * L::kSize;
   const unsigned v_bytes = static_cast<unsigned>((S - 1) * a.vs.token + dm) * L::kSize;
   const int wave_s = __builtin_amdgcn_readfirstlane(wave);
-  auto issue = [&](unsigned char* st, int key0) {  // key0 < S: the range stays positive
+  // key0 < S: the ranges stay positive. (Ids behind the last read as 0: such keys
+  // are outside every row's bounds.)
+  auto issue = [&](unsigned char* st, int* ids, int key0) {
+    if (docs != nullptr && wave_s == 0)
+      opl::buffer_copy4_lds(docs + key0, static_cast<unsigned>(S - key0) * 4, ids, lane * 4);
     const std::size_t k_at = static_cast<std::size_t>(key0) * a.ks.token;
     const std::size_t v_at = static_cast<std::size_t>(key0) * a.vs.token;
     const unsigned k_rest = k_bytes - static_cast<unsigned>(k_at) * L::kSize;
@@ -277,7 +327,9 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   half8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
-  const float scale = kRules ? 1.0f : a.rules.scale;
+  // The scores' scale in the exponent; where they are biased they get it before.
+  const float scale_of_scores = a.rules.template after<!kHalf>();
+  const float scale = kRules && a.slopes != nullptr ? 1.0f : scale_of_scores;
   const float inv_scale = 1.0f / scale;
 
   for (bool exact = false;; exact = true) {
@@ -291,7 +343,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       move_above[qc] = -INFINITY;
     }
 
-    auto body = [&](const unsigned char* cur, int key0, bool whole) {
+    auto body = [&](const unsigned char* cur, const int* ids, int key0, bool whole) {
       constexpr int kHalves = kTileKeys / 32;
       floatx4 s[kHalves][2][2];  // [32 keys][16 keys][qc]
       __builtin_amdgcn_s_setprio(1);
@@ -334,7 +386,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      if constexpr (kRules) {  // into log2 units: capped or scaled, then biased
+      if constexpr (kRules) {  // capped, then scaled to log2 units and biased
         auto each = [&](auto rule) {
 #pragma unroll
           for (int j = 0; j < kHalves; ++j)
@@ -348,14 +400,12 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         };
         if (a.rules.cap != 0.0f)
           each([&](float x, int, int) { return a.rules.template capped<!kHalf>(x); });
-        else
-          each([&](float x, int, int) { return x * a.rules.scale; });
         if (a.slopes != nullptr) {
           // distances are exact: positions are below 2^20
           const float first = static_cast<float>(key0 + 4 * quad);
           const float from[2] = {row_at - first, row_at + 16.0f - first};
           each([&](float x, int qc, int key) {
-            return fmaf(-slope, fabsf(from[qc] - static_cast<float>(key)), x);
+            return fmaf(x, scale_of_scores, -slope * fabsf(from[qc] - static_cast<float>(key)));
           });
         }
       }
@@ -364,17 +414,16 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         for (int j = 0; j < kHalves; ++j)
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
-            const int key = key0 + 32 * j + 16 * kb + 4 * quad;
-            int ids[4] = {};
-            if (docs != nullptr) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) ids[e] = max(docs[min(key + e, S - 1)], -1);
-            }
+            const int at = 32 * j + 16 * kb + 4 * quad;
+            const int key = key0 + at;
+            int4 id = make_int4(0, 0, 0, 0);
+            if (docs != nullptr) id = *reinterpret_cast<const int4*>(ids + at);
+            const int of[4] = {max(id.x, -1), max(id.y, -1), max(id.z, -1), max(id.w, -1)};
 #pragma unroll
             for (int qc = 0; qc < 2; ++qc)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                s[j][kb][qc][e] = sees(qc, key + e, ids[e]) ? s[j][kb][qc][e] : -INFINITY;
+                s[j][kb][qc][e] = sees(qc, key + e, of[e]) ? s[j][kb][qc][e] : -INFINITY;
           }
       }
       float raw[2];
@@ -415,7 +464,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 p[qc][4 * kb + e] = static_cast<_Float16>(opl::fast_exp2(
-                    kRules ? s[j][kb][qc][e] - row_max[qc] : fmaf(s[j][kb][qc][e], scale, -row_max[qc])));
+                    fmaf(s[j][kb][qc][e], scale, -row_max[qc])));
 #pragma unroll
           for (int db = 0; db < L::kDBlocks; ++db) {
             const fp16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16((OPL_LDS fp16x4*)(cur + v_base[db] + rows));
@@ -443,7 +492,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 p[qc][kb][e] = opl::fast_exp2(
-                    kRules ? s[j][kb][qc][e] - row_max[qc] : fmaf(s[j][kb][qc][e], scale, -row_max[qc]));
+                    fmaf(s[j][kb][qc][e], scale, -row_max[qc]));
                 lane_sum[qc] += p[qc][kb][e];
               }
 #pragma unroll
@@ -479,9 +528,9 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = T(0);
       }
     };
-    auto tile = [&](const unsigned char* cur, unsigned char* nxt, int t) {
+    auto tile = [&](const unsigned char* cur, const int* ids, unsigned char* nxt, int* ids_nxt, int t) {
       const int after = t < end_tile ? advance(t) : end_tile;
-      if (after < end_tile) issue(nxt, after * kTileKeys);
+      if (after < end_tile) issue(nxt, ids_nxt, after * kTileKeys);
       __builtin_amdgcn_sched_barrier(0);
       if (exact) {
         if (t < end_tile) drop_non_finite(const_cast<unsigned char*>(cur));
@@ -494,11 +543,14 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       if (t < end_tile && row0 < S &&
           (key0 < prefix || (key1 >= low(row0) && key0 <= high(row1)))) {
         bool whole = key1 < prefix || (key0 >= low(row1) && key1 <= high(row0));
+        bool within = true;
         if (docs != nullptr) {
           const int bit = key0 / 64;
-          whole = whole && ((single[bit / 32] >> (bit % 32)) & 1) != 0;
+          const bool known = bit < kMarkWords * 32;
+          within = !known || ((some[wave][bit / 32] >> (bit % 32)) & 1) != 0;
+          whole = whole && known && ((single[wave][bit / 32] >> (bit % 32)) & 1) != 0;
         }
-        body(cur, key0, whole);
+        if (within) body(cur, ids, key0, whole);
       }
       __builtin_amdgcn_s_waitcnt(0);
       if constexpr (kW == 1) {
@@ -511,14 +563,14 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     };
     int t = visit(0);
     for (int g = 0; g < group; ++g) t = visit(t + 1);
-    if (t < end_tile) issue(st0, t * kTileKeys);
+    if (t < end_tile) issue(st0, id0, t * kTileKeys);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if constexpr (kGroups == 1 || kW == 1) {
       while (t < end_tile) {  // uniform over the wavefronts that meet at the barrier
-        t = tile(st0, st1, t);
+        t = tile(st0, id0, st1, id1, t);
         if (t >= end_tile) break;
-        t = tile(st1, st0, t);
+        t = tile(st1, id1, st0, id0, t);
       }
     } else {
       // Groups of more wavefronts meet at the workgroup's barrier: all run as
@@ -526,10 +578,10 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       int lead = visit(0);
       while (lead < end_tile) {
         lead = advance(lead);
-        t = tile(st0, st1, t);
+        t = tile(st0, id0, st1, id1, t);
         if (lead >= end_tile) break;
         lead = advance(lead);
-        t = tile(st1, st0, t);
+        t = tile(st1, id1, st0, id0, t);
       }
     }
     __syncthreads();  // every stage is free
@@ -657,17 +709,92 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   }
 }
 
-template <typename T, int D, int kGroups, int kW, int kTileKeys>
+template <typename T, int D, int Dc, int kGroups, int kW, int kTileKeys>
 hipError_t launch(const MaskedArgs<T>& a, hipStream_t stream) {
   constexpr int kRows = kRowsPerWave * kW;
   const long long blocks = (a.S + kRows - 1LL) / kRows * a.bh;
   const dim3 grid(static_cast<unsigned>((blocks + kXcds - 1) / kXcds * kXcds));
   const dim3 block(kGroups * kW * opl::kWaveSize);
   if (a.rules.cap != 0.0f || a.slopes != nullptr)
-    masked_attention_kernel<T, D, kGroups, kW, kTileKeys, true><<<grid, block, 0, stream>>>(a);
+    masked_attention_kernel<T, D, Dc, kGroups, kW, kTileKeys, true><<<grid, block, 0, stream>>>(a);
   else
-    masked_attention_kernel<T, D, kGroups, kW, kTileKeys, false><<<grid, block, 0, stream>>>(a);
+    masked_attention_kernel<T, D, Dc, kGroups, kW, kTileKeys, false><<<grid, block, 0, stream>>>(a);
   return hipGetLastError();
+}
+
+// G key groups of W wavefronts, tiles of K keys: head dims up to 64, and past it.
+template <typename T, int G, int W, int K>
+hipError_t narrow(const MaskedArgs<T>& a, hipStream_t stream) {
+  return launch<T, 64, 64, G, W, K>(a, stream);
+}
+template <typename T, int G, int W, int K>
+hipError_t wide(const MaskedArgs<T>& a, hipStream_t stream) {
+  // Head dims of 65 to 96 compute on 96: fp16 B2 H16 S2999 prefix 106 -> 98 us.
+  if (a.dm <= 96) return launch<T, 128, 96, G, W, K>(a, stream);
+  return launch<T, 128, 128, G, W, K>(a, stream);
+}
+
+// Blocks of 32 to 128 query rows, and keys split between groups of wavefronts
+// where the grid of 128-row blocks does not fill the CUs' two workgroups each
+// (as attention.hip does). Measured on MI355X (us; groups, wavefronts per group,
+// tile keys), B1 unless said, "c" causal:
+//   fp16 D64    1,4,64  2,2,64  2,4,64  4,1,32     fp16 D128   1,4,64  2,2,32  2,4,64  4,2,32  4,1,32
+//   H12 S131 c    8.2     7.4     8.3     6.4      H12 S131 c   10.8     8.8    10.5     9.0     8.8
+//   H32 S500 c   13.9    10.7    12.5     8.9      H12 S500     17.2    14.4    16.2    13.2    12.6
+//   H2 S8000    109.9    68.7    86.0    53.8      H32 S500     18.0    15.1    16.7    14.1    23.3
+//   H32 S1000    20.1    17.9    18.1    23.9      H4 S4000     82.6    65.1    67.6    52.7    76.2
+//   H16 S2000 c  34.0    24.0    27.9    24.6      H32 S1000 c  29.6    24.0    25.7    26.5    45.5
+//   B4 H32 S131   8.8    10.0     9.6    12.3      H16 S2000 c  48.4    38.5    40.7    36.8    60.6
+//   H32 S2000 c  37.0    34.1    34.3    45.2      H16 S2000    48.0    44.8    40.9    55.7    88.7
+//   H32 S2000    44.6    52.8    53.4    66.8      H12 S4000 c  96.3   105.8    80.3   109.8   165.9
+//   B4 H32 S500c 16.1    19.7    19.9    27.9      H32 S2000 c  55.2    51.9    49.9    71.7   120.4
+//   B2 H32 S1000c 23.4   25.2    24.9    34.5      B2 H32 S1000c 34.7   36.1    36.1    51.8    90.1
+// Many heads of up to 192 tokens, whose second 128-row block is nearly empty:
+// 1,2,32 (B16 H32 S131 D128 23.7 against 27.3, D64 16.5 against 18.1).
+//   fp32 D64    1,4,32  2,2,32  4,1,32  1,2,32     fp32 D128   1,4,32  2,2,32  1,2,32
+//   H12 S500 c   43.0    26.1    18.1    41.8      H12 S131 c   26.3    20.8    27.9
+//   H8 S2000 c  148.9    85.3    56.2   147.7      H2 S8000     1047     607    1104
+//   H8 S2000    149.6    87.6    93.6   149.1      H32 S1000 c 142.5    97.6   149.8
+//   H16 S2000   154.4   142.1   181.9   248.8      H32 S1000   145.8   167.0   151.5
+//   H32 S2000 c 203.0   164.8   216.1   202.5      H32 S2000 c 361.7   351.0   314.5
+//   H12 S4000 window 512 (384 blocks)              B4 H32 S500 c 102.5 117.0    97.7
+//               156.7   141.3           139.9      H32 S2000   495.9   632.7   568.1
+template <typename T>
+hipError_t choose(const MaskedArgs<T>& a, hipStream_t stream) {
+  const long long blocks = (a.S + 127LL) / 128 * a.bh;
+  const long long blocks32 = (a.S + 31LL) / 32 * a.bh;
+  // Keys that a block walks, by the window.
+  const long long reach = a.window > 0 ? (a.causal ? 1LL : 2LL) * a.window + 128 : a.S;
+  const long long walk = reach < a.S ? reach : a.S;
+  if (a.dm > 64) {
+    if constexpr (sizeof(T) == 2) {
+      if (blocks32 <= 256) return wide<T, 4, 1, 32>(a, stream);
+      if (a.S <= 192 && blocks > 256) return wide<T, 1, 2, 32>(a, stream);
+      if (blocks <= 128) return wide<T, 4, 2, 32>(a, stream);
+      if (a.causal && blocks <= 256 && walk > 192) return wide<T, 2, 2, 32>(a, stream);
+      if ((blocks <= 256 && walk > 192) || (a.causal && blocks <= 512 && walk >= 1536))
+        return wide<T, 2, 4, 64>(a, stream);
+      return wide<T, 1, 4, 64>(a, stream);
+    } else {
+      if (blocks <= 128 || (a.causal && blocks <= 256 && walk > 192))
+        return wide<T, 2, 2, 32>(a, stream);
+      if (a.causal && blocks > 256 && blocks <= 512) return wide<T, 1, 2, 32>(a, stream);
+      return wide<T, 1, 4, 32>(a, stream);
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (blocks32 <= 512) return narrow<T, 4, 1, 32>(a, stream);
+    if (a.S <= 192 && blocks > 256) return narrow<T, 1, 2, 32>(a, stream);
+    if (blocks <= 256 && walk > 192) return narrow<T, 2, 2, 64>(a, stream);
+    if (a.causal && blocks <= 512 && walk >= 1536) return narrow<T, 2, 4, 64>(a, stream);
+    return narrow<T, 1, 4, 64>(a, stream);
+  } else {
+    if (blocks32 <= (a.causal ? 512 : 256)) return narrow<T, 4, 1, 32>(a, stream);
+    if (walk > 192 && (blocks <= 256 || (a.causal && blocks <= 512)))
+      return narrow<T, 2, 2, 32>(a, stream);
+    if (blocks > 256 && blocks < 512) return narrow<T, 1, 2, 32>(a, stream);
+    return narrow<T, 1, 4, 32>(a, stream);
+  }
 }
 
 template <typename T>
@@ -685,17 +812,7 @@ int masked_entry(MaskedArgs<T> a, int batch, int kv_heads, float scale, float so
   a.group = a.q_heads / kv_heads;
   a.rules = opl::ScoreRules::of(scale, softcap);
   const hipStream_t stream = static_cast<hipStream_t>(stream_handle);
-  // Blocks of 32 rows on four key groups while their grid is one round of the
-  // 256 CUs; else 128 rows per workgroup.
-  const bool few = (a.S + 31LL) / 32 * a.bh <= 256;
-  const bool wide = a.dm > 64;
-  if constexpr (sizeof(T) == 2) {
-    if (few) return wide ? launch<T, 128, 4, 1, 32>(a, stream) : launch<T, 64, 4, 1, 32>(a, stream);
-    return wide ? launch<T, 128, 1, 4, 64>(a, stream) : launch<T, 64, 1, 4, 64>(a, stream);
-  } else {
-    if (few) return wide ? launch<T, 128, 2, 2, 32>(a, stream) : launch<T, 64, 4, 1, 32>(a, stream);
-    return wide ? launch<T, 128, 1, 4, 32>(a, stream) : launch<T, 64, 1, 4, 32>(a, stream);
-  }
+  return choose(a, stream);
 }
 
 opl::MaskedStrides of(operatorlib_strides_t s) { return {s.batch, s.head, s.token}; }
