@@ -121,7 +121,7 @@ int operatorlib_rope_append_f32(
  * multiple of kv_heads; head_dim over 128; window < 0; softcap negative or not
  * finite; scale not finite or <= 0; q, cache and output not 16-byte rows; q_stride
  * below q_heads * head_dim, table_stride below max_pages; pages * kv_heads * page_size over
- * 2^32 - 1; max_pages * page_size over INT32_MAX; batch * q_heads over INT32_MAX,
+ * 2^32 - 1; max_pages * page_size over INT32_MAX - 1024; batch * q_heads over INT32_MAX,
  * or over 2^31 blocks of 64 keys in batch * kv_heads * max_pages * page_size;
  * *_ws: a workspace smaller than the query's answer, NULL, or not 256-byte
  * aligned. The queries return 0 for invalid sizes.

@@ -62,7 +62,8 @@ inline bool paged_shape_ok(const PagedShape& s, std::size_t element_bytes) {
       s.head_dim % static_cast<int>(16 / element_bytes) != 0)
     return false;
   const std::int64_t tokens = static_cast<std::int64_t>(s.max_pages) * s.page_size;
-  if (tokens > kInt32Max || static_cast<std::int64_t>(s.batch) * s.q_heads > kInt32Max)
+  // (A step past the last token still fits 32 bits.)
+  if (tokens > kInt32Max - 1024 || static_cast<std::int64_t>(s.batch) * s.q_heads > kInt32Max)
     return false;
   // batch * q_heads fits 31 bits and tokens 31 bits: no overflow in 64.
   const int tiles = (s.q_heads / s.kv_heads + kPagedHeads - 1) / kPagedHeads;

@@ -19,19 +19,22 @@
 //   * O^T has head col in the lane, like the running max and sum, so a rescale
 //     needs no exchange between lanes.
 // The matrix cores run far below their rate (at most 16 columns): the kernel
-// is bound by reading the cache. A wavefront loads tile i + 1 while it
-// computes tile i (16 KiB in flight per wavefront, 8 wavefronts per CU).
+// is bound by reading the cache. A wavefront has one set of registers for a tile
+// (K and V, 16 KiB): the next tile's K is loaded as soon as S^T is computed, its V
+// as soon as O^T is, and its page ids a tile earlier, so that loads are in
+// flight all the time.
 //
 // Work split. The host does not know the lengths. The unit of work is four
-// tiles (one per wavefront of a workgroup) of one (sequence, key head); the
-// units of all of them form one line, and workgroup w of G takes an equal,
-// contiguous piece of it, whatever mix of long and short sequences it holds.
-// Every workgroup finds its piece from the lengths (a scan of at most a few
-// of them per thread). A row (sequence, key head) that lies in one piece is
-// written at once; one cut by piece borders leaves an unnormalised O with its
-// max and sum per piece, and paged_join_kernel adds them in order of the
-// workgroups (deterministic). A piece cuts at most its first and its last
-// row: two slots of scratch per workgroup.
+// tiles (one per wavefront of a workgroup) of one row (sequence, key head).
+//   * Few units (the page table's whole width in kDirectUnits): a workgroup per
+//     unit, and the pieces of a row are the workgroups of its units.
+//   * Else the units that the lengths give form one line, and workgroup w of G
+//     takes an equal, contiguous piece of it, whatever mix of long and short
+//     sequences it holds; it finds its piece by a scan of the lengths (a few
+//     per thread). A row within one piece is written at once; a piece cuts at
+//     most its first and its last row: two slots of scratch per workgroup.
+// The pieces of a row leave unnormalised O with their max and sum, and
+// paged_join_kernel adds them in order (deterministic).
 
 #include <hip/hip_runtime.h>
 
@@ -54,8 +57,15 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-// Workgroups of a launch: two per CU of an MI355X.
+// Workgroups of a launch that shares the units out, and the most units that get
+// a workgroup each.
 constexpr int kWorkgroups = 512;
+constexpr int kDirectUnits = 512;
+// Caches from this size on are read with non-temporal loads.
+constexpr std::uint64_t kStreamBytes = std::uint64_t(384) << 20;
+// Shared-out rows below which a head's pieces are added by all wavefronts of a
+// workgroup.
+constexpr unsigned kFewRows = 64;
 // The fp16 form's probabilities are 2^(x - m + kBoost), m the running max less
 // at most kLazy: keys far below the max keep 10 more binary orders before they
 // become fp16 subnormals, and 2^(kBoost + kLazy) is far below fp16's largest.
@@ -90,9 +100,13 @@ struct PagedArgs {
   const std::int32_t* lengths;
   const float* slopes;
   T* out;
-  float* part;          // [workgroups][2][heads of a row][DP + 4]: O, max, sum
-  std::int32_t* cut;    // [rows][2]: slot of the first piece and the last workgroup
-                        // of a cut row; (0, -1) of any other
+  float* part;          // [slots][heads of a row][DP + 4]: O, max, sum; two slots per
+                        // workgroup, or (direct) one
+  std::int32_t* cut;    // [workgroups][2]: of the row that starts in the workgroup and
+                        // ends in a later one, the row and that one; else -1. Direct: NULL
+  int direct;           // units of a row that have a workgroup each; 0: shared out
+  unsigned page_mul;    // key / page_size = key * page_mul >> page_shift
+  int page_shift;
   std::int64_t q_stride, table_stride;
   int batch, q_heads, kv_heads, group, tiles_of_heads, head_dim, pages, page_size, max_pages;
   int window;
@@ -114,9 +128,16 @@ __device__ __forceinline__ int units_of(int2 r) {
   return max(1, (r.y - from + kUnitKeys - 1) / kUnitKeys);
 }
 
+template <bool kStream, typename V>
+__device__ __forceinline__ V fetch(const V* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
 // MT: 16-head operands per workgroup (group up to 16 MT). kPaged16: pages hold
 // whole 16-key blocks, so that a block's rows follow each other.
-template <typename T, int DP, int MT, bool kPaged16>
+// kStream: the cache is read past the caches' reach, with non-temporal loads.
+template <typename T, int DP, int MT, bool kPaged16, bool kStream>
 __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedArgs<T> a) {
   using S = Shape<T, DP>;
   constexpr bool kHalf = S::kHalf;
@@ -125,7 +146,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
   constexpr int kPitch = DP + 4;  // floats of a head's row in LDS: rows 16 bytes apart in the banks
   __shared__ __attribute__((aligned(16))) float joined[kWaves][kHeads][kPitch];
   __shared__ int scan[kWaves];
-  __shared__ int found[4];
+  __shared__ int found[2];
 
   const int lane = threadIdx.x % opl::kWaveSize;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / opl::kWaveSize);
@@ -133,44 +154,62 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
   const int g = lane / 16;
   const int rows_of = a.kv_heads * a.tiles_of_heads;  // rows of a sequence
 
-  // ---- this workgroup's piece of the units --------------------------------
-  const int chunk = (a.batch + kThreads - 1) / kThreads;
-  const int b_first = min(a.batch, static_cast<int>(threadIdx.x) * chunk);
-  const int b_last = min(a.batch, b_first + chunk);
-  int mine = 0;
-  for (int b = b_first; b < b_last; ++b) mine += units_of<kUnitKeys>(key_range(a, b)) * rows_of;
-  int upto = mine;  // inclusive scan over the wavefront, then over the four
+  // ---- this workgroup's piece of the units: [unit, end), of which `at` is the
+  // first of sequence b
+  int unit, end, b, at, total = 0;
+  long long G = 0;
+  if (a.direct > 0) {
+    // In this mode `at` is the first unit of the row's sequence as if every row
+    // had a.direct units.
+    const int row = blockIdx.x / a.direct;
+    b = row / rows_of;
+    at = b * rows_of * a.direct;
+    unit = blockIdx.x;
+    end = unit + 1;
+  } else {
+    const int chunk = (a.batch + kThreads - 1) / kThreads;
+    const int b_first = min(a.batch, static_cast<int>(threadIdx.x) * chunk);
+    const int b_last = min(a.batch, b_first + chunk);
+    int mine = 0;
+    for (int i = b_first; i < b_last; ++i) mine += units_of<kUnitKeys>(key_range(a, i)) * rows_of;
+    int upto = mine;  // inclusive scan over the wavefront, then over the four
 #pragma unroll
-  for (int step = 1; step < opl::kWaveSize; step *= 2) {
-    const int below = __shfl_up(upto, step);
-    if (lane >= step) upto += below;
-  }
-  if (lane == opl::kWaveSize - 1) scan[wave] = upto;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) upto += scan[w];
-    total += scan[w];
-  }
-  // (No more pieces than units: each of a cut row's workgroups has a part of it.)
-  const long long G = min(static_cast<int>(gridDim.x), total);
-  if (blockIdx.x >= G) return;
-  const int begin = static_cast<int>(static_cast<long long>(blockIdx.x) * total / G);
-  const int end = static_cast<int>((static_cast<long long>(blockIdx.x) + 1) * total / G);
-  if (begin >= upto - mine && begin < upto) {
-    int at = upto - mine, b = b_first;
-    for (;; ++b) {
-      const int u = units_of<kUnitKeys>(key_range(a, b)) * rows_of;
-      if (begin < at + u) break;
-      at += u;
+    for (int step = 1; step < opl::kWaveSize; step *= 2) {
+      const int below = __shfl_up(upto, step);
+      if (lane >= step) upto += below;
     }
-    found[0] = b;
-    found[1] = at;
+    if (lane == opl::kWaveSize - 1) scan[wave] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) upto += scan[w];
+      total += scan[w];
+    }
+    // (No more pieces than units: each of a cut row's workgroups has a part of it.)
+    G = min(static_cast<int>(gridDim.x), total);
+    if (blockIdx.x >= G) {
+      if (a.cut != nullptr && threadIdx.x == 0) a.cut[2 * blockIdx.x] = -1;
+      return;
+    }
+    const int begin = static_cast<int>(static_cast<long long>(blockIdx.x) * total / G);
+    end = static_cast<int>((static_cast<long long>(blockIdx.x) + 1) * total / G);
+    if (begin >= upto - mine && begin < upto) {
+      int first = upto - mine, i = b_first;
+      for (;; ++i) {
+        const int u = units_of<kUnitKeys>(key_range(a, i)) * rows_of;
+        if (begin < first + u) break;
+        first += u;
+      }
+      found[0] = i;
+      found[1] = first;
+    }
+    __syncthreads();
+    unit = begin;
+    b = __builtin_amdgcn_readfirstlane(found[0]);
+    at = __builtin_amdgcn_readfirstlane(found[1]);
+    total = __builtin_amdgcn_readfirstlane(total);
   }
-  __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(found[0]);
-  int at = __builtin_amdgcn_readfirstlane(found[1]);  // first unit of sequence b
+  const int begin = unit;
   const int dm = a.head_dim;
 
   // Offsets (elements) of the lane's chunks in a K and a V row; dims from dm
@@ -187,12 +226,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
     v_dim[u] = d < dm ? d : 0;
   }
 
-  int unit = begin;
   while (unit < end) {
     // ---- the row (sequence b, key head, tile of heads) that `unit` lies in
     int2 range = key_range(a, b);
-    int units = units_of<kUnitKeys>(range);
-    while (unit >= at + units * rows_of) {
+    int units = a.direct > 0 ? a.direct : units_of<kUnitKeys>(range);
+    while (unit >= at + units * rows_of) {  // (never in the direct mode)
       at += units * rows_of;
       ++b;
       range = key_range(a, b);
@@ -238,115 +276,108 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
     }
 
     const std::int32_t* table = a.page_table + static_cast<std::int64_t>(b) * a.table_stride;
-    // Page of token `key` (< n), or -1 if it is not a page.
-    auto page_of = [&](int key) {
-      const int p = table[key / a.page_size];
-      return p >= 0 && p < a.pages ? p : -1;
+    auto page_index = [&](int key) {
+      return static_cast<int>(static_cast<std::uint64_t>(static_cast<unsigned>(key)) * a.page_mul >>
+                              a.page_shift);
     };
-    // First element of a cache row.
-    auto row_start = [&](int page, int key) {
-      return (static_cast<std::int64_t>(page) * a.kv_heads + kv_head) * a.page_size +
-             key % a.page_size;
+    // Page ids of a tile's blocks (kPaged16) or of the lane's K rows; -1 behind
+    // the last token.
+    struct Pages {
+      int id[S::kSubs];
     };
-
-    // Cache rows of the lane's K and V rows in the tile from key0, and which
-    // of the lane's keys are visible (bit 4 s + r: key 16 s + 4 g + r).
-    // Rows of hidden keys are those of cache row 0.
+    auto look_up = [&](int key0) {
+      Pages p;
+#pragma unroll
+      for (int s = 0; s < S::kSubs; ++s) {
+        const int key = key0 + 16 * s + (kPaged16 ? 0 : col);
+        p.id[s] = -1;
+        if (key < n) p.id[s] = table[page_index(key)];
+      }
+      return p;
+    };
+    // Cache rows of the lane's K and V rows in the tile, and which of the lane's
+    // keys are visible (bit 4 s + r: key 16 s + 4 g + r). Hidden keys on no page
+    // read the cache's first rows.
     struct Rows {
-      std::int64_t sub[S::kSubs];            // kPaged16: first row of each block
-      std::int64_t k[S::kSubs];              // else: the lane's K rows
+      std::int64_t sub[S::kSubs];  // kPaged16: first row of each block; else the lane's K rows
       std::int64_t v[kPaged16 ? 1 : S::kVRows];
       unsigned seen;
     };
-    auto rows_at = [&](int key0) {
+    auto rows_of_tile = [&](int key0, const Pages& pages) {
       Rows r;
       r.seen = 0;
-      if constexpr (kPaged16) {
 #pragma unroll
-        for (int s = 0; s < S::kSubs; ++s) {
-          const int key = key0 + 16 * s;
-          const int page = key < n ? __builtin_amdgcn_readfirstlane(page_of(key)) : -1;
-          r.sub[s] = page >= 0 ? row_start(page, key) : 0;
-          if (page >= 0) {
+      for (int s = 0; s < S::kSubs; ++s) {
+        const int key = key0 + 16 * s + (kPaged16 ? 0 : col);
+        const int page = pages.id[s] >= 0 && pages.id[s] < a.pages ? pages.id[s] : -1;
+        r.sub[s] = page >= 0 ? (static_cast<std::int64_t>(page) * a.kv_heads + kv_head) * a.page_size +
+                                   (key - page_index(key) * a.page_size)
+                             : 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int mk = key + 4 * g + e;
-              if (mk >= lo && mk < n) r.seen |= 1u << (4 * s + e);
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int s = 0; s < S::kSubs; ++s) {
-          const int key = key0 + 16 * s + col;
-          const int page = key < n ? page_of(key) : -1;
-          r.k[s] = page >= 0 ? row_start(page, key) : 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int from = 4 * g + e;  // the lane that looked up key 16 s + 4 g + e
-            const int mk = key0 + 16 * s + from;
-            r.v[4 * s + e] = __shfl(r.k[s], from);
-            if (__shfl(page, from) >= 0 && mk >= lo && mk < n) r.seen |= 1u << (4 * s + e);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int from = 4 * g + e;  // the lane that looked up key 16 s + 4 g + e
+          const int mk = key0 + 16 * s + from;
+          if constexpr (!kPaged16) r.v[4 * s + e] = __shfl(r.sub[s], from);
+          const int its_page = kPaged16 ? page : __shfl(page, from);
+          if ((its_page >= 0) & (mk >= lo) & (mk < n)) r.seen |= 1u << (4 * s + e);
         }
       }
       return r;
     };
-    auto load = [&](typename S::Tile& t, const Rows& r) {
+    auto load_k = [&](typename S::Tile& t, const Rows& r) {
 #pragma unroll
       for (int s = 0; s < S::kSubs; ++s) {
-        const T* base = kPaged16 ? a.key_cache + r.sub[s] * dm + col * dm : a.key_cache + r.k[s] * dm;
+        const T* base = a.key_cache + r.sub[s] * dm + (kPaged16 ? col * dm : 0);
 #pragma unroll
         for (int c = 0; c < S::kSteps; ++c)
-          t.k[s][c] = *reinterpret_cast<const typename S::KFrag*>(base + k_dim[c]);
+          t.k[s][c] = fetch<kStream>(reinterpret_cast<const typename S::KFrag*>(base + k_dim[c]));
       }
+    };
+    auto load_v = [&](typename S::Tile& t, const Rows& r) {
 #pragma unroll
       for (int j = 0; j < S::kVRows; ++j) {
         const T* base = kPaged16 ? a.value_cache + r.sub[j / 4] * dm + (4 * g + j % 4) * dm
                                  : a.value_cache + r.v[kPaged16 ? 0 : j] * dm;
 #pragma unroll
         for (int u = 0; u < S::kVC; ++u)
-          t.v[j][u] = *reinterpret_cast<const typename S::VFrag*>(base + v_dim[u]);
+          t.v[j][u] = fetch<kStream>(reinterpret_cast<const typename S::VFrag*>(base + v_dim[u]));
       }
     };
-    auto compute = [&](typename S::Tile& t, unsigned seen, int key0) {
-      constexpr unsigned kAll = (1u << (4 * S::kSubs)) - 1;
-      const bool whole = __builtin_amdgcn_ballot_w64(seen != kAll) == 0;
-      if (!whole) {  // values of hidden keys are zeros: 0 x NaN is NaN
+    floatx4 x[MT][S::kSubs];
+    auto scores = [&](const typename S::Tile& t) {
 #pragma unroll
-        for (int j = 0; j < S::kVRows; ++j)
-          if (!((seen >> j) & 1)) {
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int u = 0; u < S::kVC; ++u) t.v[j][u] = typename S::VFrag{};
-          }
-      }
+        for (int s = 0; s < S::kSubs; ++s) x[mt][s] = floatx4{0, 0, 0, 0};
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        floatx4 x[S::kSubs];
+      for (int c = 0; c < S::kSteps; ++c)
 #pragma unroll
-        for (int s = 0; s < S::kSubs; ++s) x[s] = floatx4{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < S::kSteps; ++c)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int s = 0; s < S::kSubs; ++s) {
             if constexpr (kHalf) {
-              x[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[s][c], qf[mt][c], x[s], 0, 0, 0);
+              x[mt][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[s][c], qf[mt][c], x[mt][s], 0, 0, 0);
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                x[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[s][c][e], qf[mt][c][e], x[s], 0, 0, 0);
+                x[mt][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[s][c][e], qf[mt][c][e], x[mt][s], 0, 0, 0);
             }
           }
+    };
+    // Scores to probabilities (in x), with the running max and sum.
+    auto softmax = [&](unsigned seen, bool whole, int key0) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
         float top = -INFINITY;
 #pragma unroll
         for (int s = 0; s < S::kSubs; ++s)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float y = a.rules.template log2_score<!kHalf>(x[s][e]);
+            float y = a.rules.template log2_score<!kHalf>(x[mt][s][e]);
             if (a.slopes != nullptr)
               y -= slope[mt] * static_cast<float>(n - 1 - (key0 + 16 * s + 4 * g + e));
-            if (!whole && !((seen >> (4 * s + e)) & 1)) y = -INFINITY;
-            x[s][e] = y;
+            if (!whole) y = (seen >> (4 * s + e)) & 1 ? y : -INFINITY;
+            x[mt][s][e] = y;
             top = __builtin_elementwise_maximum(top, y);
           }
         top = opl::max_lane_xor32(opl::combine_xor16_f32<opl::MaxOp>(top));
@@ -359,64 +390,87 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
 #pragma unroll
           for (int i = 0; i < S::kBlocks; ++i) o[mt][i] *= alpha;
         }
-        if constexpr (kHalf) {
-          half8 p;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            p[j] = static_cast<_Float16>(opl::fast_exp2(x[j / 4][j % 4] - row_max[mt] + kBoost));
-          half8 ones;
+        for (int s = 0; s < S::kSubs; ++s)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ones[j] = static_cast<_Float16>(1.0f);
-          sums[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p, sums[mt], 0, 0, 0);
+          for (int e = 0; e < 4; ++e)
+            x[mt][s][e] = opl::fast_exp2(x[mt][s][e] - row_max[mt] + (kHalf ? kBoost : 0.0f));
+      }
+    };
+    auto values = [&](typename S::Tile& t, unsigned seen, bool whole) {
+      if (!whole) {  // values of hidden keys are zeros: 0 x NaN is NaN
 #pragma unroll
-          for (int u = 0; u < S::kVC; ++u)
+        for (int j = 0; j < S::kVRows; ++j)
+          if (!((seen >> j) & 1)) {
 #pragma unroll
-            for (int w = 0; w < S::kVW; ++w) {
-              half8 f;
+            for (int u = 0; u < S::kVC; ++u) t.v[j][u] = typename S::VFrag{};
+          }
+      }
+      if constexpr (kHalf) {
+        half8 p[MT], ones;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = t.v[j][u][w];
+        for (int j = 0; j < 8; ++j) ones[j] = static_cast<_Float16>(1.0f);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[mt][j] = static_cast<_Float16>(x[mt][j / 4][j % 4]);
+          sums[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[mt], sums[mt], 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < S::kVC; ++u)
+#pragma unroll
+          for (int w = 0; w < S::kVW; ++w) {
+            half8 f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = t.v[j][u][w];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
               o[mt][u * S::kVW + w] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[mt][u * S::kVW + w], 0, 0, 0);
-            }
-        } else {
+                  __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[mt], o[mt][u * S::kVW + w], 0, 0, 0);
+          }
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = opl::fast_exp2(x[0][e] - row_max[mt]);
-            sums[mt][0] += p;  // this lane's keys only; joined below
+            sums[mt][0] += x[mt][0][e];  // this lane's keys only; joined below
 #pragma unroll
             for (int u = 0; u < S::kVC; ++u)
 #pragma unroll
               for (int w = 0; w < S::kVW; ++w)
                 o[mt][u * S::kVW + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                    t.v[e][u][w], p, o[mt][u * S::kVW + w], 0, 0, 0);
+                    t.v[e][u][w], x[mt][0][e], o[mt][u * S::kVW + w], 0, 0, 0);
           }
-        }
       }
     };
 
     // ---- the wavefront's tiles: key0, key0 + kUnitKeys, ...
+    constexpr unsigned kAll = (1u << (4 * S::kSubs)) - 1;
     int key0 = base_key + wave * S::kKeys;
     if (key0 < last_key) {
-      typename S::Tile ta, tb;
-      Rows ra = rows_at(key0), rb;
-      load(ta, ra);
+      typename S::Tile t;
+      Rows rows = rows_of_tile(key0, look_up(key0));
+      load_k(t, rows);
+      load_v(t, rows);
+      Pages next = look_up(key0 + kUnitKeys);
       for (;;) {
         const int key1 = key0 + kUnitKeys;
-        const bool more = key1 < last_key;
-        if (more) {
-          rb = rows_at(key1);
-          load(tb, rb);
+        const unsigned seen = rows.seen;
+        const bool whole = __builtin_amdgcn_ballot_w64(seen != kAll) == 0;
+        scores(t);
+        __builtin_amdgcn_sched_barrier(0);
+        if (key1 < last_key) {
+          rows = rows_of_tile(key1, next);
+          load_k(t, rows);
+          next = look_up(key1 + kUnitKeys);
         }
-        compute(ta, ra.seen, key0);
-        if (!more) break;
-        key0 = key1 + kUnitKeys;
-        const bool again = key0 < last_key;
-        if (again) {
-          ra = rows_at(key0);
-          load(ta, ra);
-        }
-        compute(tb, rb.seen, key1);
-        if (!again) break;
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(seen, whole, key0);
+        values(t, seen, whole);
+        __builtin_amdgcn_sched_barrier(0);
+        if (key1 >= last_key) break;
+        load_v(t, rows);
+        key0 = key1;
       }
     }
 
@@ -440,9 +494,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
       }
     }
     __syncthreads();
-    const bool cut = unit != row0 || stop != row0 + units;
-    const int slot = row0 <= begin ? 0 : 1;
-    const int row_id = b * rows_of + row_in;
+    const bool cut = a.direct > 1 || unit != row0 || stop != row0 + units;
+    const int slot = a.direct > 0 ? unit : 2 * static_cast<int>(blockIdx.x) + (unit == row0 ? 1 : 0);
     for (int i = threadIdx.x; i < heads * (DP / 4); i += kThreads) {
       const int hh = i / (DP / 4);
       const int d = (i % (DP / 4)) * 4;
@@ -458,7 +511,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
         v += f * *reinterpret_cast<const floatx4*>(&joined[w][hh][d]);
       }
       if (cut) {
-        float* part = a.part + ((static_cast<std::int64_t>(blockIdx.x) * 2 + slot) * kHeads + hh) * kPitch;
+        float* part = a.part + (static_cast<std::int64_t>(slot) * kHeads + hh) * kPitch;
         *reinterpret_cast<floatx4*>(part + d) = v;
         if (d == 0) {
           part[DP] = m;
@@ -473,66 +526,124 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
         *reinterpret_cast<Out*>(a.out + (static_cast<std::int64_t>(b) * a.q_heads + head0 + hh) * dm + d) = y;
       }
     }
-    // The workgroup that starts a row says who has its pieces.
-    if (a.cut != nullptr && unit == row0 && threadIdx.x == 0) {
+    // The workgroup in which a cut row starts says where it ends (its last row).
+    if (a.cut != nullptr && stop == end && threadIdx.x == 0) {
       // workgroup of unit u: the largest w with w total / G <= u
       const long long last = (static_cast<long long>(row0 + units) * G - 1) / total;
-      a.cut[2 * row_id] = 2 * static_cast<int>(blockIdx.x) + slot;
-      a.cut[2 * row_id + 1] = cut ? static_cast<int>(last) : -1;
+      const bool starts = cut && unit == row0;
+      a.cut[2 * blockIdx.x] = starts ? b * rows_of + row_in : -1;
+      a.cut[2 * blockIdx.x + 1] = static_cast<int>(last);
     }
     unit = stop;
   }
 }
 
-// Adds the pieces of a cut row, in order: one workgroup per row. The first
-// piece is in either slot of its workgroup, the others in the first slot of
-// the workgroups after it (which start with this row).
-template <typename T, int DP, int MT>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedArgs<T> a) {
+// Adds the pieces of the rows that are in pieces, in order. Direct: a workgroup
+// per row and head. Shared-out units: a workgroup per kJoinWaves heads of the row
+// that starts in workgroup w of the launch before and ends in a later one; its
+// first piece is w's second slot, or the first if w starts with it, the others
+// are the first slots of the workgroups after w.
+// kWavesPerHead wavefronts take every kWavesPerHead-th piece of a head, a lane
+// DP / 64 dims: 1 where rows have few pieces, as there are many rows; all of
+// the workgroup's where few rows have many.
+constexpr int kJoinWaves = 8;
+template <typename T, int DP, int MT, int kWavesPerHead>
+__global__ __launch_bounds__(kJoinWaves * opl::kWaveSize) void paged_join_kernel(const PagedArgs<T> a) {
   constexpr int kHeads = 16 * MT;
   constexpr int kPitch = DP + 4;
-  const int row_id = blockIdx.x;
-  const int first = a.cut[2 * row_id];
-  const int more = a.cut[2 * row_id + 1] - first / 2;  // pieces after the first
-  if (a.cut[2 * row_id + 1] < 0) return;
+  constexpr int kDims = DP / opl::kWaveSize;
+  constexpr int kPerGroup = kJoinWaves / kWavesPerHead;  // heads of a workgroup
+  typedef float Dims __attribute__((ext_vector_type(kDims)));
+  __shared__ float top[kJoinWaves], weight[kJoinWaves], joined[kJoinWaves][DP];
   const int rows_of = a.kv_heads * a.tiles_of_heads;
+  const int head_groups = (min(kHeads, a.group) + kPerGroup - 1) / kPerGroup;
+  const int item = blockIdx.x / head_groups;  // a row, or a workgroup of the launch before
+  const int lane = threadIdx.x % opl::kWaveSize;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / opl::kWaveSize);
+  const int hh = blockIdx.x % head_groups * kPerGroup + wave / kWavesPerHead;
+  int row_id, first, second, step, count;
+  if (a.direct > 0) {
+    row_id = item;
+    first = row_id * a.direct;
+    second = first + 1;
+    step = 1;
+    count = a.direct;
+  } else {
+    row_id = a.cut[2 * item];
+    const int last = a.cut[2 * item + 1];
+    if (row_id < 0) return;
+    first = 2 * item + 1;
+    second = 2 * (item + 1);
+    step = 2;
+    count = last - item + 1;
+  }
   const int b = row_id / rows_of, row_in = row_id % rows_of;
   const int head_tile = row_in % a.tiles_of_heads;
-  const int heads = min(kHeads, a.group - head_tile * kHeads);
-  const int head0 = (row_in / a.tiles_of_heads) * a.group + head_tile * kHeads;
-  for (int i = threadIdx.x; i < heads * (DP / 4); i += kThreads) {
-    const int hh = i / (DP / 4);
-    const int d = (i % (DP / 4)) * 4;
-    if (d >= a.head_dim) continue;
-    const float* piece = a.part + (static_cast<std::int64_t>(first) * kHeads + hh) * kPitch;
-    const float* next =
-        a.part + (static_cast<std::int64_t>(first / 2 + 1) * 2 * kHeads + hh) * kPitch;
-    float m = piece[DP];
-    for (int j = 0; j < more; ++j) m = fmaxf(m, next[j * 2 * kHeads * kPitch + DP]);
-    float f = opl::fast_exp2(piece[DP] - m);
-    float l = f * piece[DP + 1];
-    floatx4 v = f * *reinterpret_cast<const floatx4*>(piece + d);
-#pragma unroll 4
-    for (int j = 0; j < more; ++j) {
-      const float* p = next + j * 2 * kHeads * kPitch;
-      f = opl::fast_exp2(p[DP] - m);
-      l += f * p[DP + 1];
-      v += f * *reinterpret_cast<const floatx4*>(p + d);
-    }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    typedef T Out __attribute__((ext_vector_type(4)));
-    Out y;
+  const bool real = hh < min(kHeads, a.group - head_tile * kHeads);
+  float m = -FLT_MAX, l = 0.0f;
+  Dims v = {};
+  constexpr int kAhead = 8;  // pieces in flight
+  for (int j0 = wave % kWavesPerHead; real && j0 < count; j0 += kWavesPerHead * kAhead) {
+    float pm[kAhead], pl[kAhead];
+    Dims po[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(v[e] * inv);
-    *reinterpret_cast<Out*>(a.out + (static_cast<std::int64_t>(b) * a.q_heads + head0 + hh) *
-                                        a.head_dim + d) = y;
+    for (int k = 0; k < kAhead; ++k) {
+      const int j = j0 + kWavesPerHead * k;
+      const int slot = j == 0 || j >= count ? first : second + (j - 1) * step;
+      const float* piece = a.part + (static_cast<std::int64_t>(slot) * kHeads + hh) * kPitch;
+      pm[k] = piece[DP];
+      pl[k] = piece[DP + 1];
+      po[k] = *reinterpret_cast<const Dims*>(piece + kDims * lane);
+      if (j >= count) pm[k] = -FLT_MAX, pl[k] = 0.0f;
+    }
+    float to = m;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) to = fmaxf(to, pm[k]);
+    const float f = opl::fast_exp2(m - to);
+    m = to;
+    l *= f;
+    v *= f;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float w = opl::fast_exp2(pm[k] - m);
+      l += w * pl[k];
+      // (An empty piece has a sum of 0 and nothing in O.)
+      if (pl[k] != 0.0f) v += w * po[k];
+    }
   }
+  if constexpr (kWavesPerHead > 1) {
+    if (lane == 0) {
+      top[wave] = m;
+      weight[wave] = l;
+    }
+    *reinterpret_cast<Dims*>(&joined[wave][kDims * lane]) = v;
+    __syncthreads();
+    if (wave != 0) return;
+    static_assert(kWavesPerHead == kJoinWaves, "one head per workgroup");
+#pragma unroll
+    for (int w = 1; w < kWavesPerHead; ++w) m = fmaxf(m, top[w]);
+    l = 0.0f;
+    v = Dims{};
+#pragma unroll
+    for (int w = 0; w < kWavesPerHead; ++w) {
+      const float f = opl::fast_exp2(top[w] - m);
+      l += f * weight[w];
+      v += f * *reinterpret_cast<const Dims*>(&joined[w][kDims * lane]);
+    }
+  }
+  if (!real || kDims * lane >= a.head_dim) return;
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const int head = (row_in / a.tiles_of_heads) * a.group + head_tile * kHeads + hh;
+  T* const out = a.out + (static_cast<std::int64_t>(b) * a.q_heads + head) * a.head_dim + kDims * lane;
+#pragma unroll
+  for (int e = 0; e < kDims; ++e) out[e] = static_cast<T>(v[e] * inv);
 }
 
 // The launch of a call and the scratch it needs.
 struct Plan {
   int workgroups;
-  bool join;           // rows can be cut
+  int direct;          // units per row with a workgroup each, 0: shared out
+  bool join;           // rows can be in pieces
   std::size_t part_bytes, bytes;
 };
 
@@ -543,29 +654,55 @@ Plan plan_of(const opl::PagedShape& s, std::size_t element_bytes) {
   const long long rows =
       static_cast<long long>(s.batch) * s.kv_heads * ((group + opl::kPagedHeads - 1) / opl::kPagedHeads);
   const long long tokens = static_cast<long long>(s.max_pages) * s.page_size;
-  const long long units = rows * ((tokens + unit - 1) / unit);
+  const long long row_units = (tokens + unit - 1) / unit;
   Plan p;
-  p.workgroups = static_cast<int>(units < kWorkgroups ? units : kWorkgroups);
-  p.join = tokens > unit;
+  p.direct = rows * row_units <= kDirectUnits ? static_cast<int>(row_units) : 0;
+  p.workgroups = static_cast<int>(p.direct ? rows * row_units : kWorkgroups);
+  p.join = row_units > 1;
   const int dp = s.head_dim > 64 ? 128 : 64;
-  p.part_bytes = p.join ? static_cast<std::size_t>(p.workgroups) * 2 * heads * (dp + 4) * sizeof(float) : 0;
-  p.bytes = p.join ? p.part_bytes + static_cast<std::size_t>(rows) * 2 * sizeof(std::int32_t) : 0;
+  const std::size_t slots = static_cast<std::size_t>(p.workgroups) * (p.direct ? 1 : 2);
+  p.part_bytes = p.join ? slots * heads * (dp + 4) * sizeof(float) : 0;
+  p.bytes = p.part_bytes +
+            (p.join && !p.direct ? static_cast<std::size_t>(p.workgroups) * 2 * sizeof(std::int32_t) : 0);
   return p;
 }
 
 template <typename T, int DP, int MT>
 hipError_t launch(PagedArgs<T> a, const Plan& plan, void* scratch, hipStream_t stream) {
   const dim3 block(kThreads);
+  a.direct = plan.direct;
   a.part = static_cast<float*>(scratch);
-  a.cut = plan.join ? reinterpret_cast<std::int32_t*>(static_cast<unsigned char*>(scratch) + plan.part_bytes)
-                    : nullptr;
-  if (a.page_size % 16 == 0)
-    paged_attention_kernel<T, DP, MT, true><<<dim3(plan.workgroups), block, 0, stream>>>(a);
-  else
-    paged_attention_kernel<T, DP, MT, false><<<dim3(plan.workgroups), block, 0, stream>>>(a);
+  a.cut = plan.join && !plan.direct
+              ? reinterpret_cast<std::int32_t*>(static_cast<unsigned char*>(scratch) + plan.part_bytes)
+              : nullptr;
+  // Caches past the 256 MiB Infinity Cache, as far as the page table can reach them.
+  const std::uint64_t row_bytes = 2ull * a.kv_heads * a.head_dim * sizeof(T);
+  const std::uint64_t held = static_cast<std::uint64_t>(a.pages) * a.page_size * row_bytes;
+  const std::uint64_t reach = static_cast<std::uint64_t>(a.max_pages) * a.page_size * a.batch * row_bytes;
+  const bool stream_past = (held < reach ? held : reach) >= kStreamBytes;
+  const dim3 grid(plan.workgroups);
+  if (a.page_size % 16 == 0) {
+    if (stream_past)
+      paged_attention_kernel<T, DP, MT, true, true><<<grid, block, 0, stream>>>(a);
+    else
+      paged_attention_kernel<T, DP, MT, true, false><<<grid, block, 0, stream>>>(a);
+  } else {
+    if (stream_past)
+      paged_attention_kernel<T, DP, MT, false, true><<<grid, block, 0, stream>>>(a);
+    else
+      paged_attention_kernel<T, DP, MT, false, false><<<grid, block, 0, stream>>>(a);
+  }
   if (plan.join) {
+    const int most = a.group < 16 * MT ? a.group : 16 * MT;
     const unsigned rows = static_cast<unsigned>(a.batch) * a.kv_heads * a.tiles_of_heads;
-    paged_join_kernel<T, DP, MT><<<dim3(rows), block, 0, stream>>>(a);
+    const dim3 join_block(kJoinWaves * opl::kWaveSize);
+    if (plan.direct)
+      paged_join_kernel<T, DP, MT, kJoinWaves><<<dim3(rows * most), join_block, 0, stream>>>(a);
+    else if (rows < kFewRows)
+      paged_join_kernel<T, DP, MT, kJoinWaves><<<dim3(plan.workgroups * most), join_block, 0, stream>>>(a);
+    else
+      paged_join_kernel<T, DP, MT, 1>
+          <<<dim3(plan.workgroups * ((most + kJoinWaves - 1) / kJoinWaves)), join_block, 0, stream>>>(a);
   }
   return hipGetLastError();
 }
@@ -587,6 +724,13 @@ int paged_entry(PagedArgs<T> a, float scale, float softcap, const opl::ScratchSo
   a.group = a.q_heads / a.kv_heads;
   a.tiles_of_heads = (a.group + opl::kPagedHeads - 1) / opl::kPagedHeads;
   a.rules = opl::ScoreRules::of(scale, softcap);
+  // floor(key / page_size) for every key below 2^31: with 2^(s - 1) < page_size
+  // <= 2^s, ceil(2^(31 + s) / page_size) fits 32 bits and errs by less than one
+  // part in key.
+  int s = 0;
+  while ((std::uint64_t(1) << s) < static_cast<std::uint64_t>(a.page_size)) ++s;
+  a.page_shift = 31 + s;
+  a.page_mul = static_cast<unsigned>(((std::uint64_t(1) << a.page_shift) + a.page_size - 1) / a.page_size);
   const Plan plan = plan_of(shape, sizeof(T));
   if (src.workspace_mode ? !opl::workspace_ok(src.data, src.bytes, plan.bytes)
                          : plan.bytes > opl::kArenaBytes)

@@ -51,13 +51,16 @@ int main() {
   expect(opl::paged_shape_ok(p, 2), false, "paged: fp16 head_dim 4");
   p = {INT_MAX, INT_MAX, INT_MAX, 128, INT_MAX, INT_MAX};
   expect(opl::paged_shape_ok(p, 2), false, "paged: everything large");
-  p = {1, 1, 1, 128, INT_MAX, 1};
-  expect(opl::paged_shape_ok(p, 2), true, "paged: one page of 2^31 - 1 tokens");
-  p = {64, 1, 1, 128, INT_MAX, 1};
-  expect(opl::paged_shape_ok(p, 2), false, "paged: 2^31 units");
-  p = {63, 1, 1, 128, INT_MAX, 1};
+  const int most_tokens = INT_MAX - 1024;
+  p = {1, 1, 1, 128, most_tokens, 1};
+  expect(opl::paged_shape_ok(p, 2), true, "paged: the largest page");
+  p = {1, 1, 1, 128, most_tokens + 1, 1};
+  expect(opl::paged_shape_ok(p, 2), false, "paged: one token more");
+  p = {65, 1, 1, 128, most_tokens, 1};
+  expect(opl::paged_shape_ok(p, 2), false, "paged: past 2^31 units");
+  p = {64, 1, 1, 128, most_tokens, 1};
   expect(opl::paged_shape_ok(p, 2), true, "paged: just below 2^31 units");
-  p = {32, 66, 2, 128, INT_MAX, 1};
+  p = {33, 66, 2, 128, most_tokens, 1};
   expect(opl::paged_shape_ok(p, 2), false, "paged: two tiles of heads count");
   expect(opl::paged_cache_ok(INT_MAX, 2, 1), true, "cache: 2^32 - 2 rows");
   expect(opl::paged_cache_ok(INT_MAX, 3, 1), false, "cache: past 2^32 rows");
