@@ -28,11 +28,11 @@ const operatorlib_half_t* half_in(const at::Tensor& t) {
   return static_cast<const operatorlib_half_t*>(caddr(t));
 }
 operatorlib_half_t* half_out(const at::Tensor& t) {
-  return t.numel() ? static_cast<operatorlib_half_t*>(t.data_ptr()) : nullptr;
+  return t.defined() ? static_cast<operatorlib_half_t*>(t.data_ptr()) : nullptr;
 }
 const float* float_in(const at::Tensor& t) { return static_cast<const float*>(caddr(t)); }
 float* float_out(const at::Tensor& t) {
-  return t.numel() ? static_cast<float*>(t.data_ptr()) : nullptr;
+  return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr;
 }
 
 // A stride of a dimension of one element is nobody's: `dense` stands for it.
@@ -116,7 +116,8 @@ std::tuple<at::Tensor, at::Tensor> rope_append_op(
   const std::int64_t qs = token_rows(in, q, "q"), ks = token_rows(in, k, "k"),
                      vs = token_rows(in, v, "v");
   at::Tensor q_out = at::empty(q.sizes(), q.options());
-  at::Tensor k_out = return_keys ? at::empty(k.sizes(), k.options()) : at::empty({0}, k.options());
+  at::Tensor k_out;  // undefined (None) unless asked for
+  if (return_keys) k_out = at::empty(k.sizes(), k.options());
   launch(in, [&](void* s) {
     return in.half()
                ? operatorlib_rope_append_f16(

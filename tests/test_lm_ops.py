@@ -112,7 +112,7 @@ def test_rope_append(ops, dtype, interleaved, tokens, heads, kv_heads, dim, rota
     kc2, vc2 = dev(kc), dev(vc)
     qo2, none = ops.rope_append(dq, dk, dv, dev(positions), dev(freq), dev(slots), kc2, vc2,
                                 axes=dev(axis), interleaved=interleaved)
-    assert none.numel() == 0 and torch.equal(qo2, qo)
+    assert none is None and torch.equal(qo2, qo)
     assert torch.equal(kc2, dkc) and torch.equal(vc2, dvc)
 
 
