@@ -101,7 +101,8 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   __shared__ unsigned some[kW][kMarkWords];   // the documents of the 64 keys and its rows may meet
   __shared__ unsigned single[kW][kMarkWords]; // its rows and the 64 keys are one document
   __shared__ int span[kW][3];                 // least and greatest document of its rows, 1 if it has one
-  __shared__ int again;
+  __shared__ float2 ends[kGroups > 1 ? kGroups * kW : 1][kRowsPerWave];  // max and sum of a row
+  __shared__ bool poisoned[kGroups * kW];
 
   // ---- which rows of which head: XCD x takes a contiguous range of the work,
   // heads in order (the query heads of a key head follow each other), heaviest
@@ -322,7 +323,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 
   // ---- state: lane l holds query 16 qc + col, dims 16 db + 4 quad + e of O^T
   floatx4 o[2][L::kDBlocks];
-  float row_max[2], move_above[2], lane_sum[2];
+  float row_max[2], move_above[2], lane_sum[2], row_sum[2];
   floatx4 sums[2];
   half8 ones;
 #pragma unroll
@@ -332,7 +333,8 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   const float scale = kRules && a.slopes != nullptr ? 1.0f : scale_of_scores;
   const float inv_scale = 1.0f / scale;
 
-  for (bool exact = false;; exact = true) {
+  bool exact = false;  // uniform over the workgroup
+  for (;;) {
 #pragma unroll
     for (int qc = 0; qc < 2; ++qc) {
 #pragma unroll
@@ -584,63 +586,57 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         t = tile(st1, id1, st0, id0, t);
       }
     }
-    __syncthreads();  // every stage is free
-    if (exact) break;
-    // A NaN in O: a non-finite value was multiplied by a hidden key's 0, or is
-    // seen.
-    bool bad = false;
+    // Every lane of a row has its max and sum; the groups exchange them. A NaN in
+    // the sum of a wavefront's O: a non-finite value was multiplied by a hidden
+    // key's 0, or is seen (or infinities of both signs are).
+    float all[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int qc = 0; qc < 2; ++qc)
+    for (int qc = 0; qc < 2; ++qc) {
+      row_sum[qc] = kHalf ? sums[qc][0]
+                          : opl::sum_lane_xor32(opl::combine_xor16_f32<opl::SumOp>(lane_sum[qc]));
+      if (kGroups > 1 && quad == 0)
+        ends[group * kW + wave][16 * qc + col] = make_float2(row_max[qc], row_sum[qc]);
 #pragma unroll
       for (int db = 0; db < L::kDBlocks; ++db)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= o[qc][db][e] != o[qc][db][e];
-    if (threadIdx.x == 0) again = 0;
-    __syncthreads();
-    if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) again = 1;
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(again) == 0) break;
+        for (int e = 0; e < 4; ++e) all[e] += o[qc][db][e];
+    }
+    const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+    const bool bad = __builtin_amdgcn_ballot_w64(sum != sum) != 0;
+    if (lane == 0) poisoned[threadIdx.x / opl::kWaveSize] = bad && !exact;
+    __syncthreads();  // every stage is free
+    bool again = false;
+#pragma unroll
+    for (int i = 0; i < kGroups * kW; ++i) again |= poisoned[i];
+    if (!__builtin_amdgcn_readfirstlane(again)) break;
+    exact = true;
+    __syncthreads();  // (all have read the flags)
   }
   // ---- join the groups, normalise, store whole rows through LDS
-  float row_sum[2], coef[2];
-#pragma unroll
-  for (int qc = 0; qc < 2; ++qc)
-    row_sum[qc] = kHalf ? sums[qc][0]
-                        : opl::sum_lane_xor32(opl::combine_xor16_f32<opl::SumOp>(lane_sum[qc]));
+  float coef[2];
   auto inverse = [](float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; };
-  if constexpr (kGroups > 1) {
-    constexpr int kSlots = kThreads;
-    float* const xs = reinterpret_cast<float*>(stage0);
-    const int slot = threadIdx.x;
 #pragma unroll
-    for (int qc = 0; qc < 2; ++qc) {
-      xs[qc * kSlots + slot] = row_max[qc];
-      xs[(2 + qc) * kSlots + slot] = row_sum[qc];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int qc = 0; qc < 2; ++qc) {
+  for (int qc = 0; qc < 2; ++qc) {
+    if constexpr (kGroups > 1) {
+      float2 of[kGroups];
       float m = -FLT_MAX, l = 0.0f;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-        m = fmaxf(m, xs[qc * kSlots + (g * kW + wave) * opl::kWaveSize + lane]);
-#pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const int sl = (g * kW + wave) * opl::kWaveSize + lane;
-        l += xs[(2 + qc) * kSlots + sl] * opl::fast_exp2(xs[qc * kSlots + sl] - m);
+        of[g] = ends[g * kW + wave][16 * qc + col];
+        m = fmaxf(m, of[g].x);
       }
-      coef[qc] = opl::fast_exp2(row_max[qc] - m) * inverse(l);
-    }
-    __syncthreads();
-  } else {
 #pragma unroll
-    for (int qc = 0; qc < 2; ++qc) coef[qc] = inverse(row_sum[qc]);
+      for (int g = 0; g < kGroups; ++g) l += of[g].y * opl::fast_exp2(of[g].x - m);
+      coef[qc] = opl::fast_exp2(row_max[qc] - m) * inverse(l);
+    } else {
+      coef[qc] = inverse(row_sum[qc]);
+    }
   }
 #pragma unroll
   for (int qc = 0; qc < 2; ++qc)
 #pragma unroll
     for (int db = 0; db < L::kDBlocks; ++db) o[qc][db] *= coef[qc];
-  if (__builtin_amdgcn_readfirstlane(again) != 0) {
+  if (exact) {
     // The non-finite values go to the rows that see their keys, after the
     // weights (infinity times a weight of 0 is NaN); one group adds them, as
     // the groups' O are summed.
@@ -682,7 +678,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         to[r * kQuads + ((4 * db + quad) ^ (r % kQuads))] = o[qc][db];
       }
   }
-  __syncthreads();
+  if constexpr (kGroups > 1) __syncthreads();  // (else a wavefront reads what it wrote)
   // Each wavefront stores 32 / kGroups rows of its block's kGroups copies.
   constexpr int kLanes = kQuads;                       // lanes per row
   constexpr int kRowsPerStore = opl::kWaveSize / kLanes;
