@@ -45,6 +45,7 @@
 #include <type_traits>
 
 #include "common.hpp"
+#include "divide.hpp"
 #include "lm_validate.hpp"
 #include "operatorlib/lm_c.h"
 #include "scores.hpp"
@@ -105,8 +106,7 @@ struct PagedArgs {
   std::int32_t* cut;    // [workgroups][2]: of the row that starts in the workgroup and
                         // ends in a later one, the row and that one; else -1. Direct: NULL
   int direct;           // units of a row that have a workgroup each; 0: shared out
-  unsigned page_mul;    // key / page_size = key * page_mul >> page_shift
-  int page_shift;
+  opl::Divider page_of; // key / page_size
   std::int64_t q_stride, table_stride;
   int batch, q_heads, kv_heads, group, tiles_of_heads, head_dim, pages, page_size, max_pages;
   int window;
@@ -276,10 +276,6 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
     }
 
     const std::int32_t* table = a.page_table + static_cast<std::int64_t>(b) * a.table_stride;
-    auto page_index = [&](int key) {
-      return static_cast<int>(static_cast<std::uint64_t>(static_cast<unsigned>(key)) * a.page_mul >>
-                              a.page_shift);
-    };
     // Page ids of a tile's blocks (kPaged16) or of the lane's K rows; -1 behind
     // the last token.
     struct Pages {
@@ -291,7 +287,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
       for (int s = 0; s < S::kSubs; ++s) {
         const int key = key0 + 16 * s + (kPaged16 ? 0 : col);
         p.id[s] = -1;
-        if (key < n) p.id[s] = table[page_index(key)];
+        if (key < n) p.id[s] = table[a.page_of.quotient(key)];
       }
       return p;
     };
@@ -311,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAr
         const int key = key0 + 16 * s + (kPaged16 ? 0 : col);
         const int page = pages.id[s] >= 0 && pages.id[s] < a.pages ? pages.id[s] : -1;
         r.sub[s] = page >= 0 ? (static_cast<std::int64_t>(page) * a.kv_heads + kv_head) * a.page_size +
-                                   (key - page_index(key) * a.page_size)
+                                   (key - a.page_of.quotient(key) * a.page_size)
                              : 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -724,13 +720,7 @@ int paged_entry(PagedArgs<T> a, float scale, float softcap, const opl::ScratchSo
   a.group = a.q_heads / a.kv_heads;
   a.tiles_of_heads = (a.group + opl::kPagedHeads - 1) / opl::kPagedHeads;
   a.rules = opl::ScoreRules::of(scale, softcap);
-  // floor(key / page_size) for every key below 2^31: with 2^(s - 1) < page_size
-  // <= 2^s, ceil(2^(31 + s) / page_size) fits 32 bits and errs by less than one
-  // part in key.
-  int s = 0;
-  while ((std::uint64_t(1) << s) < static_cast<std::uint64_t>(a.page_size)) ++s;
-  a.page_shift = 31 + s;
-  a.page_mul = static_cast<unsigned>(((std::uint64_t(1) << a.page_shift) + a.page_size - 1) / a.page_size);
+  a.page_of = opl::Divider::by(a.page_size);
   const Plan plan = plan_of(shape, sizeof(T));
   if (src.workspace_mode ? !opl::workspace_ok(src.data, src.bytes, plan.bytes)
                          : plan.bytes > opl::kArenaBytes)
