@@ -62,8 +62,12 @@ constexpr int kWaves = 4;
 // a workgroup each.
 constexpr int kWorkgroups = 512;
 constexpr int kDirectUnits = 512;
-// Caches from this size on are read with non-temporal loads.
-constexpr std::uint64_t kStreamBytes = std::uint64_t(384) << 20;
+// Caches from this size on, three quarters of the 256 MiB Infinity Cache, are read
+// with non-temporal loads: they cannot stay there from one step to the next
+// beside anything else. Batch of 64 (1.18 GB) 221 -> 195 us (6.0 TB/s), one
+// sequence of 131072 tokens (537 MB) 107 -> 97; 263 MB 62.7 -> 57.4 after other
+// work, 52.4 -> 57.1 where the step before had left them there; 137 MB 33.3 -> 36.7.
+constexpr std::uint64_t kStreamBytes = std::uint64_t(192) << 20;
 // Shared-out rows below which a head's pieces are added by all wavefronts of a
 // workgroup.
 constexpr unsigned kFewRows = 64;
@@ -671,7 +675,7 @@ hipError_t launch(PagedArgs<T> a, const Plan& plan, void* scratch, hipStream_t s
   a.cut = plan.join && !plan.direct
               ? reinterpret_cast<std::int32_t*>(static_cast<unsigned char*>(scratch) + plan.part_bytes)
               : nullptr;
-  // Caches past the 256 MiB Infinity Cache, as far as the page table can reach them.
+  // The cache's bytes, as far as the page table can reach them.
   const std::uint64_t row_bytes = 2ull * a.kv_heads * a.head_dim * sizeof(T);
   const std::uint64_t held = static_cast<std::uint64_t>(a.pages) * a.page_size * row_bytes;
   const std::uint64_t reach = static_cast<std::uint64_t>(a.max_pages) * a.page_size * a.batch * row_bytes;

@@ -120,3 +120,18 @@ def masked_attention(q, k, v, causal=False, window=0, softcap=0.0, slopes=None, 
                 out[b, h] = _rows(q[b, h], kh, vh, seen, distance, scale, softcap,
                                   None if slopes is None else slopes[h])
     return out
+
+
+# Shapes that reach every instance of masked_attention: (dtype, head_dim,
+# (groups, wavefronts, tile keys), batch, heads, sequence, causal, window).
+_WIDE_F16 = [((4, 1, 32), 1, 2, 150, True, 0), ((1, 2, 32), 9, 16, 150, True, 0), ((4, 2, 32), 1, 24, 500, False, 0),
+             ((2, 2, 32), 1, 20, 1000, True, 0), ((2, 4, 64), 1, 20, 1000, False, 0),
+             ((2, 4, 64), 1, 20, 1600, True, 0), ((1, 4, 64), 1, 40, 1000, False, 90)]
+_NARROW_F16 = [((4, 1, 32), 1, 2, 150, True, 0), ((1, 2, 32), 9, 16, 150, False, 0), ((2, 2, 64), 1, 20, 1000, False, 0),
+               ((2, 4, 64), 1, 20, 1600, True, 0), ((1, 4, 64), 1, 40, 1000, True, 0)]
+_WIDE_F32 = [((2, 2, 32), 1, 2, 150, True, 0), ((2, 2, 32), 1, 20, 1000, True, 0), ((1, 2, 32), 1, 40, 1000, True, 0),
+             ((1, 4, 32), 1, 40, 1000, False, 0)]
+_NARROW_F32 = [((4, 1, 32), 1, 2, 150, True, 0), ((2, 2, 32), 1, 20, 500, False, 0), ((1, 2, 32), 1, 40, 1000, False, 0),
+               ((1, 4, 32), 1, 64, 1000, False, 90)]
+MASKED_ROUTES = ([("f16", d, *r) for d in (128, 80) for r in _WIDE_F16] + [("f16", 64, *r) for r in _NARROW_F16]
+                 + [("f32", d, *r) for d in (128, 80) for r in _WIDE_F32] + [("f32", 64, *r) for r in _NARROW_F32])

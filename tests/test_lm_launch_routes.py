@@ -1,0 +1,122 @@
+"""Which kernel instances the language-model entry points launch, on the host
+(tests/host/lm_launches.cpp: the sources compiled for the host, the HIP launch
+calls answered there). The calls below reach every instance that is compiled,
+and both sides of each rule; tests/test_lm_routes.py runs the same shapes on the
+GPU."""
+
+from __future__ import annotations
+
+import os
+import re
+import shutil
+import subprocess
+from concurrent.futures import ThreadPoolExecutor
+from pathlib import Path
+
+import pytest
+
+from lm_reference import MASKED_ROUTES
+
+HERE = Path(__file__).resolve().parent
+REPO = HERE.parent
+CSRC = REPO / "orin-cuda-operator-library_amd" / "csrc"
+HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+
+@pytest.fixture(scope="module")
+def program(tmp_path_factory):
+    if not Path(HIPCC).exists() or shutil.which("g++") is None:
+        pytest.skip("needs hipcc and g++")
+    out = tmp_path_factory.mktemp("lm_launches")
+
+    def compile_host(src):
+        obj = out / (src.name + ".o")
+        subprocess.run([HIPCC, "-x", "hip", "--cuda-host-only", "-O1", "-fPIC", "-std=c++17",
+                        "--offload-arch=gfx950", f"-I{CSRC}", f"-I{REPO / 'include'}", "-c", str(src),
+                        "-o", str(obj)], check=True, capture_output=True, text=True, timeout=600)
+        return str(obj)
+
+    sources = [CSRC / f"{n}.hip" for n in ("rope_append", "paged_attention", "masked_attention", "scratch")]
+    with ThreadPoolExecutor(5) as pool:
+        objs = list(pool.map(compile_host, [*sources, HERE / "host" / "lm_launches.cpp"]))
+    exe = out / "lm_launches"
+    # The HIP calls that no launch makes stay unresolved.
+    subprocess.run(["g++", *objs, "-Wl,--unresolved-symbols=ignore-all", "-Wl,--allow-multiple-definition",
+                    "-o", str(exe)], check=True, capture_output=True, text=True, timeout=120)
+    return exe
+
+
+def ask(program, calls):
+    text = "".join(" ".join(map(str, c)) + "\n" for c in calls)
+    proc = subprocess.run([str(program)], input=text, capture_output=True, text=True, check=True, timeout=60)
+    answers = []
+    for line in proc.stdout.splitlines():
+        status, *names = line.split()
+        assert status == "0", line
+        answers.append(names)
+    assert len(answers) == len(calls)
+    return answers
+
+
+def registered(program, kernel):
+    out = subprocess.run([str(program), "names"], capture_output=True, text=True, check=True, timeout=60).stdout
+    return {n for n in out.split() if kernel in n}
+
+
+RULES = [(c, b) for c in (0, 1) for b in (0, 1)]
+
+
+def test_every_masked_attention_instance_is_reached(program):
+    calls, want = [], []
+    for dtype, dim, instance, batch, heads, seq, causal, window in MASKED_ROUTES:
+        for capped, biased in RULES:
+            calls.append(("masked", dtype, batch, heads, heads // 2, seq, dim, int(causal), window, capped, biased))
+            want.append(instance)
+    reached = set()
+    for call, names, instance in zip(calls, ask(program, calls), want):
+        assert len(names) == 1, names
+        numbers = [int(i) for i in re.findall(r"Li(\d+)E", names[0])]
+        assert numbers[2:5] == list(instance), (call, names)
+        reached.add(names[0])
+    assert reached == registered(program, "masked_attention_kernel")
+
+
+def test_every_paged_attention_instance_is_reached(program):
+    calls = [("paged", dtype, batch, heads, kv, dim, page, width, pages)
+             for dtype in ("f16", "f32") for dim in (64, 128) for heads, kv in ((4, 2), (40, 2))
+             for page in (16, 24) for batch, width, pages in ((1, 1, 4), (1, 60, 70), (1, 4000, 9000), (600, 4000, 2000000))]
+    answers = ask(program, calls)
+    # One step covers the table: no join. (A page of 24 tokens or 16 is one step.)
+    assert all((len(a) == 1) == (c[7] == 1) for c, a in zip(calls, answers))
+    for kernel in ("paged_attention_kernel", "paged_join_kernel"):
+        assert {n for a in answers for n in a if kernel in n} == registered(program, kernel)
+
+
+def test_every_rope_append_instance_is_reached(program):
+    calls = [("rope", dtype, tokens, 32, 8, 64, rotary, interleaved, offset)
+             for dtype in ("f16", "f32") for tokens in (1, 100000) for rotary, offset in ((64, 0), (64, 1), (20, 0))
+             for interleaved in (0, 1)]
+    reached = {n for a in ask(program, calls) for n in a}
+    assert reached == registered(program, "rope_append_kernel")
+
+
+def test_masked_attention_rules_on_both_sides(program):
+    """(groups, wavefronts per group, tile keys) on both sides of each line."""
+    cases = [("f16", 128, 1, 8, 1024, 1, 0, (4, 1, 32)), ("f16", 128, 1, 8, 1025, 1, 0, (4, 2, 32)),
+             ("f16", 128, 1, 16, 1024, 0, 0, (4, 2, 32)), ("f16", 128, 1, 17, 1024, 0, 0, (2, 4, 64)),
+             ("f16", 128, 1, 17, 1024, 1, 0, (2, 2, 32)), ("f16", 128, 1, 32, 1024, 0, 0, (2, 4, 64)),
+             ("f16", 128, 1, 33, 1024, 0, 0, (1, 4, 64)), ("f16", 128, 1, 33, 1535, 1, 0, (1, 4, 64)),
+             ("f16", 128, 1, 33, 1536, 1, 0, (2, 4, 64)), ("f16", 128, 1, 33, 1536, 1, 1000, (1, 4, 64)),
+             ("f16", 128, 2, 100, 192, 1, 0, (1, 2, 32)), ("f16", 128, 2, 100, 193, 1, 0, (1, 4, 64)),
+             ("f16", 64, 1, 16, 1024, 1, 0, (4, 1, 32)), ("f16", 64, 1, 17, 1024, 1, 0, (2, 2, 64)),
+             ("f16", 64, 1, 33, 1024, 1, 0, (1, 4, 64)), ("f16", 64, 1, 17, 1024, 1, 64, (1, 4, 64)),
+             ("f32", 128, 1, 16, 1024, 0, 0, (2, 2, 32)), ("f32", 128, 1, 17, 1024, 0, 0, (1, 4, 32)),
+             ("f32", 128, 1, 32, 1024, 1, 0, (2, 2, 32)), ("f32", 128, 1, 33, 1024, 1, 0, (1, 2, 32)),
+             ("f32", 128, 1, 65, 1024, 1, 0, (1, 4, 32)), ("f32", 64, 1, 8, 1024, 0, 0, (4, 1, 32)),
+             ("f32", 64, 1, 9, 1024, 0, 0, (2, 2, 32)), ("f32", 64, 1, 16, 1024, 1, 0, (4, 1, 32)),
+             ("f32", 64, 1, 33, 1024, 0, 0, (1, 2, 32)), ("f32", 64, 1, 64, 1024, 0, 0, (1, 4, 32)),
+             ("f32", 64, 1, 64, 1024, 1, 0, (2, 2, 32)), ("f32", 64, 1, 65, 1024, 1, 0, (1, 4, 32))]
+    calls = [("masked", t, b, h, h, s, d, c, w, 0, 0) for t, d, b, h, s, c, w, _ in cases]
+    for case, names in zip(cases, ask(program, calls)):
+        numbers = [int(i) for i in re.findall(r"Li(\d+)E", names[0])]
+        assert tuple(numbers[2:5]) == case[-1], (case, names)
