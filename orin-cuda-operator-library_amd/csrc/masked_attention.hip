@@ -121,8 +121,13 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   if (w >= total) return;
   int bh = w / q_blocks;
   int qb = q_blocks - 1 - w % q_blocks;
-  if (a.causal) {
-    const int g = max(1, kCausalGroupSlots / q_blocks);
+  if (a.causal || a.documents != nullptr) {
+    // Heads whose blocks are taken together: about the slots of an XCD, all of the
+    // XCD's where its work is two rounds or less, or with documents, whose heavy
+    // blocks are anywhere (11 documents in 8000 tokens, 32 heads: 178 -> 153 us; 3 in
+    // 2000 of a batch of 4, every key of a document visible: 191 -> 159).
+    const bool all = a.documents != nullptr || per_xcd <= 2 * kCausalGroupSlots;
+    const int g = max(1, (all ? per_xcd : kCausalGroupSlots) / q_blocks);
     if (g > 1) {
       const int first = w / (g * q_blocks) * g;
       const int heads = min(g, a.bh - first);
