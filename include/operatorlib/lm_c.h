@@ -71,9 +71,10 @@ int operatorlib_lm_abi_version(void);
  * element keeps one or the other's.
  *
  * Errors: a NULL pointer other than axes, k_out, and, with rotary_dim 0,
- * positions and frequencies; key_cache equal to value_cache; a size <= 0 (rotary_dim: < 0); rotary_dim odd or
- * over head_dim; a stride below heads * head_dim; pages * page_size over
- * INT32_MAX; tokens * heads over what a launch of 2^31 workgroups holds.
+ * positions and frequencies; key_cache and value_cache overlapping; a size <= 0
+ * (rotary_dim: < 0); rotary_dim odd or over head_dim; a stride below
+ * heads * head_dim; pages * page_size over INT32_MAX; a token of more than
+ * 2^31 - 2^20 - 1 elements (q, k and v); tokens over 2^24 - 8.
  * Any head_dim and alignment is accepted; 16-byte rows and a rotary_dim / 2
  * (interleaved: rotary_dim) that is a multiple of 8 (fp16) or 4 (fp32) are
  * the fast form.
@@ -118,10 +119,11 @@ int operatorlib_rope_append_f32(
  * the grid splits a sequence; the query depends on the sizes only.
  *
  * Errors: a NULL pointer other than slopes; a size <= 0; q_heads not a
- * multiple of kv_heads; head_dim over 128; window < 0; softcap negative or not
- * finite; scale not finite or <= 0; q, cache and output not 16-byte rows; q_stride
- * below q_heads * head_dim, table_stride below max_pages; pages * kv_heads * page_size over
- * 2^32 - 1; max_pages * page_size over INT32_MAX - 1024; batch * q_heads over INT32_MAX,
+ * multiple of kv_heads; head_dim over 128; window < 0; scale outside
+ * [2^-100, 2^100]; softcap not 0 and softcap or scale / softcap outside of that;
+ * q, cache and output not 16-byte rows; q_stride below q_heads * head_dim,
+ * table_stride below max_pages; pages * kv_heads * page_size over 2^32 - 1;
+ * max_pages * page_size over INT32_MAX - 1024; batch * q_heads over INT32_MAX,
  * or over 2^31 blocks of 64 keys in batch * kv_heads * max_pages * page_size;
  * *_ws: a workspace smaller than the query's answer, NULL, or not 256-byte
  * aligned. The queries return 0 for invalid sizes.
@@ -183,10 +185,13 @@ typedef struct {
  * the probabilities to fp16 for the product with v.
  *
  * Errors: a NULL pointer other than slopes, documents, prefixes; a size <= 0;
- * q_heads not a multiple of kv_heads; head_dim over 128; window < 0; softcap
- * negative or not finite; scale not finite or <= 0; tensors not 16-byte rows; a
- * token stride below head_dim, or a negative stride; 64 tokens or a whole head
- * of a tensor spanning 2^31 bytes or more; sequence over 2^20; batch * q_heads * blocks of 32 queries over INT32_MAX.
+ * q_heads not a multiple of kv_heads; head_dim over 128; window < 0; scale
+ * outside [2^-100, 2^100]; softcap not 0 and softcap or scale / softcap outside of
+ * that; tensors not 16-byte rows; a token stride below head_dim, or a negative
+ * stride; 64 tokens or a whole head of a tensor spanning 2^31 bytes or more;
+ * sequence over 2^20; batch * q_heads * blocks of 32 queries over 2^24 - 8.
+ * (q, k and v may repeat rows, with batch and head strides of 0; the rows of
+ * output must be apart, which is not checked.)
  */
 int operatorlib_masked_attention_f16(
     const operatorlib_half_t* q, operatorlib_strides_t q_strides, const operatorlib_half_t* k,

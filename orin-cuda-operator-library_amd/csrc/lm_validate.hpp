@@ -13,6 +13,9 @@ namespace opl {
 
 constexpr std::int64_t kInt32Max = std::numeric_limits<std::int32_t>::max();
 
+// A launch holds less than 2^32 threads: workgroups of 256 that always fit.
+constexpr std::int64_t kMostWorkgroups = (1 << 24) - 8;
+
 // Sizes, strides and flags of a rope_append call.
 struct RopeShape {
   std::int64_t q_stride, k_stride, v_stride;
@@ -20,21 +23,27 @@ struct RopeShape {
 };
 
 inline bool rope_shape_ok(const RopeShape& s) {
-  if (s.tokens <= 0 || s.q_heads <= 0 || s.kv_heads <= 0 || s.head_dim <= 0 || s.pages <= 0 ||
+  if (s.tokens <= 0 || s.tokens > kMostWorkgroups || s.q_heads <= 0 || s.kv_heads <= 0 || s.head_dim <= 0 || s.pages <= 0 ||
       s.page_size <= 0 || s.rotary_dim < 0 || s.rotary_dim % 2 != 0 || s.rotary_dim > s.head_dim)
     return false;
   if (s.rotary_dim > 0 && s.position_rows <= 0) return false;
   if (static_cast<std::int64_t>(s.pages) * s.page_size > kInt32Max) return false;
   const std::int64_t q_row = static_cast<std::int64_t>(s.q_heads) * s.head_dim;
   const std::int64_t kv_row = static_cast<std::int64_t>(s.kv_heads) * s.head_dim;
-  // A token's elements are counted in 32 bits by the kernel.
-  if (q_row > kInt32Max || kv_row > kInt32Max || q_row + 2 * kv_row > kInt32Max) return false;
+  // A token's elements are counted in 32 bits by the kernel, in steps of up to
+  // 3 x 1024 workgroups of 256.
+  if (q_row > kInt32Max || kv_row > kInt32Max || q_row + 2 * kv_row > kInt32Max - (1 << 20))
+    return false;
   return s.q_stride >= q_row && s.k_stride >= kv_row && s.v_stride >= kv_row;
 }
 
-// The rules that turn a dot product into a score.
+// The rules that turn a dot product into a score. The kernels multiply by
+// scale, by scale / softcap and by softcap, each times up to 2 log2 e, and by their
+// inverses: none may leave the range of fp32.
+inline bool within_rules(float x) { return x >= 0x1p-100f && x <= 0x1p100f; }
 inline bool score_rules_ok(float scale, int window, float softcap) {
-  return std::isfinite(scale) && scale > 0.0f && window >= 0 && std::isfinite(softcap) && softcap >= 0.0f;
+  return within_rules(scale) && window >= 0 &&
+         (softcap == 0.0f || (within_rules(softcap) && within_rules(scale / softcap)));
 }
 
 inline bool aligned_rows(const void* p, std::size_t element_bytes, std::int64_t stride) {
@@ -93,7 +102,7 @@ inline bool masked_shape_ok(const MaskedShape& s, std::size_t element_bytes) {
       s.head_dim % static_cast<int>(16 / element_bytes) != 0)
     return false;
   const std::int64_t heads = static_cast<std::int64_t>(s.batch) * s.q_heads;
-  return heads <= kInt32Max && heads * ((s.sequence + 31) / 32) <= kInt32Max - 8;
+  return heads <= kMostWorkgroups && heads * ((s.sequence + 31) / 32) <= kMostWorkgroups;
 }
 
 struct MaskedStrides {

@@ -74,7 +74,8 @@ struct MaskedArgs {
   opl::ScoreRules rules;
 };
 
-// What becomes of the scores.
+// What becomes of the scores. kBoth: capped in the precise form, and biased if
+// there are slopes; it takes fp16's caps past kSigmaCap too.
 enum Rules { kScaled, kCapped, kBiased, kBoth };
 
 template <typename T, int D, int kGroups, int kW, int kTileKeys>
@@ -93,6 +94,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   constexpr bool kHalf = L::kSize == 2;
   constexpr bool kCaps = kRules == kCapped || kRules == kBoth;
   constexpr bool kBiases = kRules == kBiased || kRules == kBoth;
+  constexpr bool kPrecise = !kHalf || kRules == kBoth;  // (how a score is capped)
   using Frag = typename std::conditional<kHalf, half8, floatx4>::type;
   constexpr int kRows = kW * kRowsPerWave;
   constexpr int kThreads = kW * kGroups * opl::kWaveSize;
@@ -279,7 +281,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     return ((near) | (key < prefix)) & (id == row_doc[qc]);
   };
   const float row_at = static_cast<float>(wave_row0 + col);
-  const float slope = kBiases ? a.slopes[head] * opl::kLog2e : 0.0f;
+  const float slope = kBiases && a.slopes != nullptr ? a.slopes[head] * opl::kLog2e : 0.0f;
 
   // ---- copies of a tile: byte offset of the lane's chunks, swizzled
   constexpr int kNoData = static_cast<int>(0x80000000u);
@@ -339,7 +341,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
   // The scores' scale in the exponent; where they are biased they get it before.
-  const float scale_of_scores = kCaps ? a.rules.template after<!kHalf>() : a.rules.scale;
+  const float scale_of_scores = kCaps ? a.rules.template after<kPrecise>() : a.rules.scale;
   const float scale = kBiases ? 1.0f : scale_of_scores;
   const float inv_scale = 1.0f / scale;
 
@@ -408,7 +410,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 float x = s[j][kb][qc][e];
-                if constexpr (kCaps) x = a.rules.template capped<!kHalf>(x);
+                if constexpr (kCaps) x = a.rules.template capped<kPrecise>(x);
                 if constexpr (kBiases) {  // (positions are below 2^20: exact)
                   const float from = row_at - static_cast<float>(key0 + 4 * quad);
                   x = fmaf(x, scale_of_scores, -slope * fabsf(from + (16 * qc - 32 * j - 16 * kb - e)));
@@ -729,7 +731,8 @@ hipError_t launch(const MaskedArgs<T>& a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((blocks + kXcds - 1) / kXcds * kXcds));
   const dim3 block(kGroups * kW * opl::kWaveSize);
   const bool capped = a.rules.cap != 0.0f, biased = a.slopes != nullptr;
-  if (capped && biased)
+  const bool wide_cap = sizeof(T) == 2 && a.rules.wide_cap();
+  if (capped && (biased || wide_cap))
     masked_attention_kernel<T, D, Dc, kGroups, kW, kTileKeys, kBoth><<<grid, block, 0, stream>>>(a);
   else if (capped)
     masked_attention_kernel<T, D, Dc, kGroups, kW, kTileKeys, kCapped><<<grid, block, 0, stream>>>(a);

@@ -232,7 +232,6 @@ hipError_t launch(RopeArgs<T> a, bool interleaved, hipStream_t stream) {
   long long parts = (items + kThreads - 1) / kThreads;
   const long long spread = (1024 + a.tokens - 1) / a.tokens;
   if (parts > spread) parts = spread;
-  if (parts * a.tokens > opl::kInt32Max) return hipErrorInvalidValue;
   a.parts = static_cast<int>(parts);
   const auto divider = [](long long n) { return opl::Divider::by(n > 0 ? static_cast<int>(n) : 1); };
   a.of_part = divider(parts);
@@ -263,8 +262,12 @@ int rope_entry(RopeArgs<T> a, int interleaved, int pages, void* stream_handle) {
                                 a.page_size};
   if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.slots == nullptr ||
       a.q_out == nullptr || a.key_cache == nullptr || a.value_cache == nullptr ||
-      a.key_cache == a.value_cache || !opl::rope_shape_ok(shape))
+      !opl::rope_shape_ok(shape))
     return hipErrorInvalidValue;
+  // (a cache's bytes fit 63 bits: slots and a token's elements fit 31 each)
+  const std::uint64_t cache_bytes = static_cast<std::uint64_t>(pages) * a.page_size * a.kv_heads * a.head_dim * sizeof(T);
+  const auto key_at = reinterpret_cast<std::uintptr_t>(a.key_cache), value_at = reinterpret_cast<std::uintptr_t>(a.value_cache);
+  if ((key_at < value_at ? value_at - key_at : key_at - value_at) < cache_bytes) return hipErrorInvalidValue;
   if (a.rotary_dim > 0 && (a.positions == nullptr || a.frequencies == nullptr))
     return hipErrorInvalidValue;
   a.cache_slots = pages * a.page_size;

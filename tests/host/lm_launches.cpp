@@ -87,7 +87,7 @@ int main(int argc, char**) {
       const operatorlib_strides_t q = {int64_t(h) * s * d, int64_t(s) * d, d};
       const operatorlib_strides_t k = {int64_t(hk) * s * d, int64_t(s) * d, d};
       const float* slopes = biased ? f32(5) : nullptr;
-      const float cap = capped ? 30.0f : 0.0f;
+      const float cap = capped == 2 ? 1e6f : capped ? 30.0f : 0.0f;
       status = half ? operatorlib_masked_attention_f16(f16(1), q, f16(2), k, f16(3), k, slopes,
                                                        nullptr, nullptr, f16(4), q, b, h, hk, s, d,
                                                        0.1f, causal, window, cap, nullptr)
@@ -96,16 +96,18 @@ int main(int argc, char**) {
                                                        0.1f, causal, window, cap, nullptr);
     } else if (std::strcmp(op, "paged") == 0) {
       int b, h, hk, d, page, width, pages;
-      if (std::scanf("%d %d %d %d %d %d %d", &b, &h, &hk, &d, &page, &width, &pages) != 7) return 1;
+      float cap;
+      if (std::scanf("%d %d %d %d %d %d %d %f", &b, &h, &hk, &d, &page, &width, &pages, &cap) != 8)
+        return 1;
       const size_t ws = size_t(1) << 40;
       status = half ? operatorlib_paged_attention_f16_ws(f16(1), int64_t(h) * d, f16(2), f16(3),
                                                          i32(6), width, i32(7), nullptr, f16(4), b,
                                                          h, hk, d, pages, page, width, 0.1f, 0,
-                                                         0.0f, f32(9), ws, nullptr)
+                                                         cap, f32(9), ws, nullptr)
                     : operatorlib_paged_attention_f32_ws(f32(1), int64_t(h) * d, f32(2), f32(3),
                                                          i32(6), width, i32(7), nullptr, f32(4), b,
                                                          h, hk, d, pages, page, width, 0.1f, 0,
-                                                         0.0f, f32(9), ws, nullptr);
+                                                         cap, f32(9), ws, nullptr);
     } else {
       int t, h, hk, d, rotary, interleaved, offset;
       if (std::scanf("%d %d %d %d %d %d %d", &t, &h, &hk, &d, &rotary, &interleaved, &offset) != 7)

@@ -71,15 +71,20 @@ int main() {
   expect(opl::score_rules_ok(inf, 0, 0.0f), false, "rules: scale");
   expect(opl::score_rules_ok(1.0f, 0, -inf), false, "rules: softcap");
   expect(opl::score_rules_ok(1.0f, -1, 0.0f), false, "rules: window");
+  expect(opl::score_rules_ok(0x1p-100f, 0, 0.0f), true, "rules: the least scale");
+  expect(opl::score_rules_ok(0x1p-101f, 0, 0.0f), false, "rules: below the least scale");
+  expect(opl::score_rules_ok(0x1p50f, 0, 0x1p-50f), true, "rules: the largest scale / softcap");
+  expect(opl::score_rules_ok(0x1p50f, 0, 0x1p-51f), false, "rules: past the largest scale / softcap");
+  expect(opl::score_rules_ok(0x1p-50f, 0, 0x1p51f), false, "rules: below the least scale / softcap");
 
   opl::MaskedShape m = {2, 4, 2, 80, 64};
   expect(opl::masked_shape_ok(m, 2), true, "masked");
   m = {INT_MAX, INT_MAX, INT_MAX, 1 << 20, 128};
   expect(opl::masked_shape_ok(m, 2), false, "masked: everything large");
-  m = {1, 65535, 65535, 1 << 20, 128};
-  expect(opl::masked_shape_ok(m, 2), true, "masked: just below 2^31 blocks");
-  m = {1, 65536, 65536, 1 << 20, 128};
-  expect(opl::masked_shape_ok(m, 2), false, "masked: 2^31 blocks");
+  m = {1, 511, 511, 1 << 20, 128};
+  expect(opl::masked_shape_ok(m, 2), true, "masked: just below 2^24 blocks");
+  m = {1, 512, 512, 1 << 20, 128};
+  expect(opl::masked_shape_ok(m, 2), false, "masked: 2^24 blocks");
   m = {1, 1, 1, 1 << 20, 64};
   alignas(16) static char memory[32];
   const opl::MaskedStrides at = {0, 0, 1016}, past = {0, 0, 1024}, most = {far & ~7, far & ~7, far & ~7};

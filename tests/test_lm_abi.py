@@ -85,7 +85,9 @@ ROPE_BAD = [dict([(n, None)]) for n in ("q", "k", "v", "positions", "frequencies
                                         "key_cache", "value_cache")]
 ROPE_BAD += [{n: x} for n in ("tokens", "q_heads", "kv_heads", "head_dim", "pages", "page_size") for x in (0, -1)]
 ROPE_BAD += [dict(rows=0), dict(rotary_dim=-2), dict(rotary_dim=127), dict(rotary_dim=130), dict(qs=511),
-             dict(ks=255), dict(vs=255), dict(value_cache=FAKE), dict(pages=2 ** 27),
+             dict(ks=255), dict(vs=255), dict(value_cache=FAKE), dict(value_cache=FAKE + 16 * 2 * 128),
+             dict(value_cache=FAKE - 16), dict(tokens=2 ** 24 - 7), dict(pages=2 ** 27),
+             dict(q_heads=2 ** 31 - 2 ** 20 - 4, head_dim=1, rotary_dim=0, qs=2 ** 31),
              dict(pages=2 ** 31 - 1, page_size=2 ** 31 - 1), dict(q_heads=2 ** 24, qs=2 ** 31),
              dict(q_heads=2 ** 31 - 1, kv_heads=2 ** 31 - 1, qs=2 ** 60, ks=2 ** 60, vs=2 ** 60),
              dict(tokens=2 ** 31 - 1, q_heads=2 ** 31 - 1, qs=2 ** 40)]
@@ -107,8 +109,9 @@ def paged(lib, t, ws=False):
     return Call(getattr(lib, f"operatorlib_paged_attention_{t}{'_ws' if ws else ''}"), args)
 
 
-RULES_BAD = [dict(scale=x) for x in (0.0, -1.0, math.inf, math.nan)]
-RULES_BAD += [dict(softcap=x) for x in (-1.0, math.inf, math.nan)] + [dict(window=-1)]
+RULES_BAD = [dict(scale=x) for x in (0.0, -1.0, math.inf, math.nan, 2.0 ** -101, 2.0 ** 101)]
+RULES_BAD += [dict(softcap=x) for x in (-1.0, math.inf, math.nan, 2.0 ** -101, 2.0 ** 101)] + [dict(window=-1)]
+RULES_BAD += [dict(scale=2.0 ** 60, softcap=2.0 ** -60), dict(scale=2.0 ** -60, softcap=2.0 ** 60)]
 PAGED_BAD = [{n: None} for n in ("q", "key_cache", "value_cache", "page_table", "lengths", "output")]
 PAGED_BAD += [{n: x} for n in ("batch", "q_heads", "kv_heads", "head_dim", "pages", "page_size", "max_pages")
               for x in (0, -1)]

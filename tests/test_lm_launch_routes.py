@@ -63,7 +63,7 @@ def registered(program, kernel):
     return {n for n in out.split() if kernel in n}
 
 
-RULES = [(c, b) for c in (0, 1) for b in (0, 1)]
+RULES = [(c, b) for c in (0, 1, 2) for b in (0, 1)]  # (2: a cap of 1e6)
 
 
 def test_every_masked_attention_instance_is_reached(program):
@@ -82,9 +82,10 @@ def test_every_masked_attention_instance_is_reached(program):
 
 
 def test_every_paged_attention_instance_is_reached(program):
-    calls = [("paged", dtype, batch, heads, kv, dim, page, width, pages)
+    calls = [("paged", dtype, batch, heads, kv, dim, page, width, pages, cap)
              for dtype in ("f16", "f32") for dim in (64, 128) for heads, kv in ((4, 2), (40, 2))
-             for page in (16, 24) for batch, width, pages in ((1, 1, 4), (1, 60, 70), (1, 4000, 9000), (600, 4000, 2000000))]
+             for page in (16, 24) for batch, width, pages in ((1, 1, 4), (1, 60, 70), (1, 4000, 9000), (600, 4000, 2000000))
+             for cap in (0, 30, 1e6)]
     answers = ask(program, calls)
     # One step covers the table: no join. (A page of 24 tokens or 16 is one step.)
     assert all((len(a) == 1) == (c[7] == 1) for c, a in zip(calls, answers))
@@ -98,6 +99,15 @@ def test_every_rope_append_instance_is_reached(program):
              for interleaved in (0, 1)]
     reached = {n for a in ask(program, calls) for n in a}
     assert reached == registered(program, "rope_append_kernel")
+
+
+@pytest.mark.parametrize("cap,wide", [(0, False), (1024, False), (1025, True)])
+def test_paged_attention_caps_on_both_sides(program, cap, wide):
+    """(The last parameter of the fp16 instances; fp32 has one form.)"""
+    for dtype in ("f16", "f32"):
+        [names] = ask(program, [("paged", dtype, 1, 4, 2, 128, 16, 60, 70, cap)])
+        [name] = [n for n in names if "paged_attention_kernel" in n]
+        assert re.findall(r"Lb(\d)E", name)[-1] == str(int(wide and dtype == "f16")), name
 
 
 def test_masked_attention_rules_on_both_sides(program):

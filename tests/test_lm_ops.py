@@ -245,6 +245,40 @@ def test_paged_attention_rules(ops, dtype, page, window, softcap, bias):
     check_attention(run_paged(ops, t, slopes=slopes, **kw), want, dtype)
 
 
+# Small caps, both sides of the one past which fp16 takes the precise form, and caps
+# that no score comes near.
+CAPS = [2.0 ** -40, 0.02, 1024.0, 1025.0, 30000.0, 1e6, 2.0 ** 80]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("softcap", CAPS)
+@pytest.mark.parametrize("bias", [False, True])
+def test_paged_attention_caps(ops, dtype, softcap, bias):
+    t = paged_inputs(21, dtype, [1, 40, 300], 8, 2, 64, 16)
+    kw = dict(softcap=softcap, slopes=2.0 ** -torch.arange(1.0, 9.0) if bias else None)
+    check_attention(run_paged(ops, t, **kw), ref.paged_attention(*t, **kw), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("softcap", CAPS)
+@pytest.mark.parametrize("bias", [False, True])
+def test_masked_attention_caps(ops, dtype, softcap, bias):
+    t = masked_inputs(22, dtype, 2, 8, 2, 200, 64)
+    kw = dict(causal=True, softcap=softcap, slopes=2.0 ** -torch.arange(1.0, 9.0) if bias else None)
+    check_attention(run_masked(ops, t, **kw), ref.masked_attention(*t, **kw), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 1e-6])
+def test_attention_small_scales(ops, dtype, scale):
+    """Every visible key weighs the same."""
+    t = paged_inputs(23, dtype, [1, 40, 300], 8, 2, 64, 16)
+    check_attention(run_paged(ops, t, scale=scale), ref.paged_attention(*t, scale=scale), dtype)
+    t = masked_inputs(24, dtype, 2, 8, 2, 200, 64)
+    check_attention(run_masked(ops, t, causal=True, scale=scale),
+                    ref.masked_attention(*t, causal=True, scale=scale), dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_paged_attention_many_sequences(ops, dtype):
     """More sequences than a workgroup has threads, most of them short."""

@@ -414,3 +414,19 @@ def test_torch_refusals(ops):
     raises(rope(b=h(3, 3, 64), c=h(3, 3, 64)), "do not agree")
     raises(rope(c=h(3, 2, 32)), "same shape")
     raises(rope(a=h(3, 64, 4).transpose(1, 2)), "contiguous")
+
+
+def test_most_workgroups(ops):
+    """As many tokens and blocks as a launch takes."""
+    tokens = 2 ** 24 - 8
+    q, k, v = (torch.arange(tokens, device="cuda").remainder(n).half().view(tokens, 1, 1) for n in (1999, 2003, 2011))
+    nothing = torch.zeros(0, device="cuda")
+    slots = torch.arange(tokens - 1, -1, -1, dtype=torch.int32, device="cuda")
+    caches = [torch.zeros(tokens // 8, 1, 8, 1, dtype=torch.float16, device="cuda") for _ in range(2)]
+    qo, ko = ops.rope_append(q, k, v, slots, nothing, slots, *caches, return_keys=True)
+    assert torch.equal(qo, q) and torch.equal(ko, k)
+    assert torch.equal(caches[0].flatten(), k.flatten().flip(0)) and torch.equal(caches[1].flatten(), v.flatten().flip(0))
+    for dtype in (torch.float16, torch.float32):
+        q = torch.ones(8, 2 ** 21 - 1, 1, 8, dtype=dtype, device="cuda")
+        v = torch.arange(q.numel(), device="cuda").remainder(2039).to(dtype).view(q.shape)
+        assert torch.equal(ops.masked_attention(q, q, v), v)  # of one key
