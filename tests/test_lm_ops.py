@@ -523,3 +523,31 @@ def test_prompt_then_decode(ops, dtype, softcap, bias, window):
                                     slopes=None if slopes is None else slopes.cpu())[0].transpose(0, 1)
         check_attention(whole, want, dtype)
         check_attention(one, want[-1:], dtype)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (40, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 24])
+def test_paged_attention_wide_cap_instances(ops, heads, kv_heads, dim, page):
+    """Caps past kSigmaCap have instances of their own; also of a cache that is streamed."""
+    t = paged_inputs(25, "f16", [70, 600], heads, kv_heads, dim, page)
+    check_attention(run_paged(ops, t, softcap=1e5), ref.paged_attention(*t, softcap=1e5), "f16")
+    q, kc, vc, table, lengths = (dev(x) for x in t)
+    wide = (200 << 20) // (2 * kv_heads * page * dim * 2) + 1   # pages of 200 MiB
+    kw, vw = (torch.zeros(wide, *kc.shape[1:], dtype=kc.dtype, device="cuda") for _ in range(2))
+    kw[-kc.shape[0]:], vw[-kc.shape[0]:] = kc, vc
+    reach = torch.zeros(2, wide, dtype=torch.int32, device="cuda")
+    reach[:, :table.shape[1]] = table + (wide - kc.shape[0])
+    got = ops.paged_attention(q, kw, vw, reach, lengths, softcap=1e5)
+    check_attention(got, ref.paged_attention(*t, softcap=1e5), "f16")
+
+
+@pytest.mark.parametrize("route", [r for r in ref.MASKED_ROUTES if r[0] == "f16"],
+                         ids=lambda r: "-".join(map(str, r)).replace(" ", ""))
+def test_masked_attention_wide_cap_is_no_cap(ops, route):
+    """Every launch shape, without slopes: 1e6 tanh(s / 1e6) differs from s by s^3 / 3e12."""
+    _, dim, _, batch, heads, seq, causal, window = route
+    g = torch.Generator(device="cuda").manual_seed(seq)
+    q, k, v = (torch.randn(batch, h, seq, dim, generator=g, device="cuda").half() for h in (heads, heads // 2, heads // 2))
+    got = ops.masked_attention(q, k, v, causal=causal, window=window, softcap=1e6)
+    check_attention(got, ops.masked_attention(q, k, v, causal=causal, window=window).double().cpu(), "f16")
