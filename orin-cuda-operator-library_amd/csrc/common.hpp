@@ -180,6 +180,14 @@ __device__ __forceinline__ void buffer_copy16_lds(const void* base, unsigned byt
       (__attribute__((address_space(3))) void*)dst, 16, voffset, 0, 0, Aux);
 }
 
+// 16 bytes per lane into registers; zeros where voffset is not within `bytes`.
+__device__ __forceinline__ auto buffer_load16(const void* base, unsigned bytes, int voffset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0), bytes,
+                                        kBufferFlags),
+      voffset, 0, 0);
+}
+
 // The same for 4 bytes per lane, into LDS at dst + 4 * lane.
 __device__ __forceinline__ void buffer_copy4_lds(const void* base, unsigned bytes, void* dst,
                                                  int voffset) {

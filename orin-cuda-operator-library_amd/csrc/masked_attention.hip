@@ -166,6 +166,22 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     return a.window > 0 && a.window < S - i ? i + a.window - 1 : S - 1;
   };
 
+  // ---- Q^T operand. (Nothing is done to it on arrival: the reads of documents and
+  // the first tile are issued behind it.)
+  constexpr int kNoData = static_cast<int>(0x80000000u);
+  Frag qf[2][L::kSteps];
+#pragma unroll
+  for (int qc = 0; qc < 2; ++qc) {
+    const int row = min(wave_row0 + 16 * qc + col, S - 1) * static_cast<int>(a.qs.token);
+    const unsigned bytes = static_cast<unsigned>((S - 1) * a.qs.token + dm) * L::kSize;
+#pragma unroll
+    for (int c = 0; c < L::kSteps; ++c) {
+      const int dim = L::kSubK * c + L::kElems * quad;
+      const auto x = opl::buffer_load16(qh, bytes, dim < dm ? (row + dim) * L::kSize : kNoData);
+      qf[qc][c] = __builtin_bit_cast(Frag, x);
+    }
+  }
+
   // ---- the tiles that the block visits
   const int last_row = min(q0 + kRows, S) - 1;
   const int prefix_tiles = (prefix + kTileKeys - 1) / kTileKeys;
@@ -258,18 +274,11 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     return min(t, end_tile);
   };
 
-  // ---- Q^T operand, masks of the lane's rows
-  Frag qf[2][L::kSteps];
+  // ---- masks of the lane's rows
   int row_lo[2], row_span[2], row_doc[2];
 #pragma unroll
   for (int qc = 0; qc < 2; ++qc) {
     const int i = min(wave_row0 + 16 * qc + col, S - 1);
-#pragma unroll
-    for (int c = 0; c < L::kSteps; ++c) {
-      const int dim = L::kSubK * c + L::kElems * quad;
-      qf[qc][c] = *reinterpret_cast<const Frag*>(qh + i * a.qs.token + (dim < dm ? dim : 0));
-      if (dim >= dm) qf[qc][c] = Frag{};
-    }
     row_lo[qc] = low(i);
     row_span[qc] = high(i) - row_lo[qc];
     row_doc[qc] = 0;  // without documents every key's id is read as 0
@@ -284,7 +293,6 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   const float slope = kBiases && a.slopes != nullptr ? a.slopes[head] * opl::kLog2e : 0.0f;
 
   // ---- copies of a tile: byte offset of the lane's chunks, swizzled
-  constexpr int kNoData = static_cast<int>(0x80000000u);
   int k_src[kCopies], v_src[kCopies];
 #pragma unroll
   for (int j = 0; j < kCopies; ++j) {
@@ -679,30 +687,38 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       }
     }
   }
-  constexpr int kBlockBytes = kRowsPerWave * D * 4;
+  // (One group stores what it has: fp16 is rounded before the exchange.)
+  typedef typename std::conditional<kGroups == 1, T, float>::type Stage;
+  typedef Stage StageFour __attribute__((ext_vector_type(4)));
+  constexpr int kBlockBytes = kRowsPerWave * D * static_cast<int>(sizeof(Stage));
   constexpr int kPerArray = kArray / kBlockBytes;
   static_assert(kPerArray >= 1 && kGroups * kW <= 2 * kPerArray, "blocks fit the stage arrays");
-  auto block = [&](int index) -> floatx4* {
-    return reinterpret_cast<floatx4*>(index < kPerArray ? stage0 + index * kBlockBytes
-                                                        : stage1 + (index - kPerArray) * kBlockBytes);
+  auto block = [&](int index) -> StageFour* {
+    return reinterpret_cast<StageFour*>(index < kPerArray ? stage0 + index * kBlockBytes
+                                                          : stage1 + (index - kPerArray) * kBlockBytes);
   };
-  constexpr int kQuads = D / 4;  // groups of 4 dims in a row
+  constexpr int kQuads = D / 4;                        // groups of 4 dims in a row
+  constexpr int kQuadsPerLane = L::kElems / 4;         // of a lane's 16-byte store
+  auto swizzle = [](int row) { return row * kQuadsPerLane % kQuads; };
   {
-    floatx4* const to = block(group * kW + wave);
+    StageFour* const to = block(group * kW + wave);
 #pragma unroll
     for (int qc = 0; qc < 2; ++qc)
 #pragma unroll
       for (int db = 0; db < L::kDBlocks; ++db) {
         const int r = 16 * qc + col;
-        to[r * kQuads + ((4 * db + quad) ^ (r % kQuads))] = o[qc][db];
+        StageFour x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = static_cast<Stage>(o[qc][db][e]);
+        to[r * kQuads + ((4 * db + quad) ^ swizzle(r))] = x;
       }
   }
   if constexpr (kGroups > 1) __syncthreads();  // (else a wavefront reads what it wrote)
   // Each wavefront stores 32 / kGroups rows of its block's kGroups copies.
-  constexpr int kLanes = kQuads;                       // lanes per row
+  constexpr int kLanes = D / L::kElems;                // lanes per row
   constexpr int kRowsPerStore = opl::kWaveSize / kLanes;
   constexpr int kWaveRows = kRowsPerWave / kGroups;
-  typedef T Out __attribute__((ext_vector_type(4)));
+  typedef T Out __attribute__((ext_vector_type(L::kElems)));
   const int v = group * kW + wave;
   const int bw = v / kGroups;
   const int cc = lane % kLanes;
@@ -710,17 +726,19 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
 #pragma unroll
   for (int i = 0; i < kWaveRows / kRowsPerStore; ++i) {
     const int row = (v % kGroups) * kWaveRows + kRowsPerStore * i + lane / kLanes;
-    const int at = row * kQuads + (cc ^ (row % kQuads));
-    floatx4 x = block(bw)[at];
+    Out y;
 #pragma unroll
-    for (int g = 1; g < kGroups; ++g) x += block(g * kW + bw)[at];
-    const int token = q0 + kRowsPerWave * bw + row;
-    if (token < S && 4 * cc < dm) {
-      Out y;
+    for (int j = 0; j < kQuadsPerLane; ++j) {
+      const int at = row * kQuads + ((cc * kQuadsPerLane + j) ^ swizzle(row));
+      StageFour x = block(bw)[at];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(x[e]);
-      *reinterpret_cast<Out*>(obase + token * a.os.token + 4 * cc) = y;
+      for (int g = 1; g < kGroups; ++g) x += block(g * kW + bw)[at];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[4 * j + e] = static_cast<T>(x[e]);
     }
+    const int token = q0 + kRowsPerWave * bw + row;
+    if (token < S && L::kElems * cc < dm)
+      *reinterpret_cast<Out*>(obase + token * a.os.token + L::kElems * cc) = y;
   }
 }
 
