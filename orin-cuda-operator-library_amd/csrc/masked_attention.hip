@@ -170,17 +170,21 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   // the first tile are issued behind it.)
   constexpr int kNoData = static_cast<int>(0x80000000u);
   Frag qf[2][L::kSteps];
+  int row_doc[2] = {0, 0};  // without documents every key's id is read as 0
+  auto read_q = [&] {
 #pragma unroll
-  for (int qc = 0; qc < 2; ++qc) {
-    const int row = min(wave_row0 + 16 * qc + col, S - 1) * static_cast<int>(a.qs.token);
-    const unsigned bytes = static_cast<unsigned>((S - 1) * a.qs.token + dm) * L::kSize;
+    for (int qc = 0; qc < 2; ++qc) {
+      const int row = min(wave_row0 + 16 * qc + col, S - 1) * static_cast<int>(a.qs.token);
+      const unsigned bytes = static_cast<unsigned>((S - 1) * a.qs.token + dm) * L::kSize;
 #pragma unroll
-    for (int c = 0; c < L::kSteps; ++c) {
-      const int dim = L::kSubK * c + L::kElems * quad;
-      const auto x = opl::buffer_load16(qh, bytes, dim < dm ? (row + dim) * L::kSize : kNoData);
-      qf[qc][c] = __builtin_bit_cast(Frag, x);
+      for (int c = 0; c < L::kSteps; ++c) {
+        const int dim = L::kSubK * c + L::kElems * quad;
+        const auto x = opl::buffer_load16(qh, bytes, dim < dm ? (row + dim) * L::kSize : kNoData);
+        qf[qc][c] = __builtin_bit_cast(Frag, x);
+      }
     }
-  }
+  };
+  if (docs == nullptr) read_q();
 
   // ---- the tiles that the block visits
   const int last_row = min(q0 + kRows, S) - 1;
@@ -223,12 +227,16 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
     const int chunks = min((end_tile * kTileKeys + 63) / 64, kMarkWords * 32);
     int c0 = threadIdx.x / opl::kWaveSize * 64;
     Ids keys = ids_of(min(c0 + lane, chunks - 1));
+    read_q();
     int least_row = i < S && id >= 0 ? id : 0x7fffffff, most_row = i < S ? max(id, -1) : -1;
 #pragma unroll
     for (int step = 1; step < kRowsPerWave; step *= 2) {
       least_row = min(least_row, __shfl_xor(least_row, step));
       most_row = max(most_row, __shfl_xor(most_row, step));
     }
+#pragma unroll
+    for (int qc = 0; qc < 2; ++qc)
+      row_doc[qc] = __shfl(id >= 0 ? id : -2, 16 * qc + col);  // (-2: no key's id)
     const bool padded = __builtin_amdgcn_ballot_w64(i < S && id < 0) != 0;
     if (group == 0 && lane == 0) {
       span[wave][0] = least_row;
@@ -275,14 +283,12 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
   };
 
   // ---- masks of the lane's rows
-  int row_lo[2], row_span[2], row_doc[2];
+  int row_lo[2], row_span[2];
 #pragma unroll
   for (int qc = 0; qc < 2; ++qc) {
     const int i = min(wave_row0 + 16 * qc + col, S - 1);
     row_lo[qc] = low(i);
     row_span[qc] = high(i) - row_lo[qc];
-    row_doc[qc] = 0;  // without documents every key's id is read as 0
-    if (docs != nullptr) row_doc[qc] = docs[i] >= 0 ? docs[i] : -2;  // no key's id
   }
   // Whether the lane's row of block qc sees a key whose document is id (-1: none).
   auto sees = [&](int qc, int key, int id) -> bool {
@@ -365,7 +371,7 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
       move_above[qc] = -INFINITY;
     }
 
-    auto body = [&](const unsigned char* cur, const int* ids, int key0, bool whole) {
+    auto body = [&](const unsigned char* cur, const int* ids, int key0, bool whole, bool bounds) {
       constexpr int kHalves = kTileKeys / 32;
       floatx4 s[kHalves][2][2];  // [32 keys][16 keys][qc]
       __builtin_amdgcn_s_setprio(1);
@@ -428,7 +434,22 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (!whole) {
+      if (bounds) {  // three instructions a score instead of eight (window 320: 88.8 -> 82.0 us)
+#pragma unroll
+        for (int qc = 0; qc < 2; ++qc) {
+          const int from = key0 + 4 * quad - row_lo[qc];
+#pragma unroll
+          for (int j = 0; j < kHalves; ++j)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[j][kb][qc][e] = static_cast<unsigned>(from + 32 * j + 16 * kb + e) <=
+                                          static_cast<unsigned>(row_span[qc])
+                                      ? s[j][kb][qc][e]
+                                      : -INFINITY;
+        }
+      } else if (!whole) {
 #pragma unroll
         for (int j = 0; j < kHalves; ++j)
 #pragma unroll
@@ -578,7 +599,8 @@ void masked_attention_kernel(const MaskedArgs<T> a) {
           (key0 < prefix || (key1 >= low(row0) && key0 <= high(row1)))) {
         bool whole = key1 < prefix || (key0 >= low(row1) && key1 <= high(row0));
         whole = whole && one != 0;
-        if (within != 0) body(cur, ids, key0, whole);
+        const bool bounds = !whole && one != 0 && key0 >= prefix;  // alone decide
+        if (within != 0) body(cur, ids, key0, whole, bounds);
       }
       __builtin_amdgcn_s_waitcnt(0);
       if constexpr (kW == 1) {
