@@ -27,6 +27,17 @@
 //     ends with a NaN, the block runs again with the non-finite values of V
 //     taken for zeros, and then adds them to the rows that see their keys.
 //     Blocks without a NaN pay one test.
+//
+// Measured on MI355X, fp16, 32 + 8 heads of 128:
+//   * 8192 tokens, causal: 523 us, 1050 TFLOP/s of the visible products (a large
+//     library product runs at 1189): matrix cores and exponentials hardly overlap, as in
+//     attention.hip. Capped 612 to 631 us (870 to 900 TFLOP/s), biased 590: bound by the
+//     vector units, with three transcendental instructions a capped score.
+//   * 11 documents in 8000 tokens: 151 us where the products alone take 67. A
+//     workgroup of 10 tiles spends 11 k of its 69 k cycles before the first one (marks
+//     5.8 k, queries, first copy) and 3 k behind the last, partial tiles cost a quarter
+//     more than whole ones, and the last heavy blocks run when the others are done
+//     (a tenth of the workgroups in the last 22 us).
 
 #include <hip/hip_runtime.h>
 

@@ -35,6 +35,16 @@
 //     most its first and its last row: two slots of scratch per workgroup.
 // The pieces of a row leave unnormalised O with their max and sum, and
 // paged_join_kernel adds them in order (deterministic).
+//
+// Measured on MI355X, fp16, head_dim 128:
+//   * 64 sequences of 1 to 8192 tokens, 32 + 8 heads (1.18 GB of cache): 194 us,
+//     6.1 TB/s (a 1 GiB copy moves 5.2); 512 workgroups are the two that fit a CU
+//     with 2 x 16 KiB in flight per SIMD (three a CU spilled registers).
+//   * 2 of 131072 tokens, 16 + 2 heads (263 MB): 57.6 us, of which the join is 6.
+//   * 1 of 1000 tokens, 32 + 8 heads: 10.1 us, the chain length -> page -> K -> V ->
+//     partial, twice a launch (1.7), and the join's two reads. The last workgroup of
+//     a row joining instead of a launch took 11.6 us (15.3 with agent-scope
+//     fences); looking pages up before the lengths arrive gained nothing.
 
 #include <hip/hip_runtime.h>
 
@@ -59,7 +69,9 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 // Workgroups of a launch that shares the units out, and the most units that get
-// a workgroup each.
+// a workgroup each: what one round holds. (32 + 8 heads, one sequence of 4000 tokens:
+// direct 10.4 us, shared out 14.0; of 8100: 12.9, 16.5; 4 of 2000: 12.8, 17.9. In two
+// rounds, one of 16000 tokens: direct 23.3, shared out 23.0.)
 constexpr int kWorkgroups = 512;
 constexpr int kDirectUnits = 512;
 // Caches from this size on, three quarters of the 256 MiB Infinity Cache, are read
@@ -68,9 +80,10 @@ constexpr int kDirectUnits = 512;
 // sequence of 131072 tokens (537 MB) 107 -> 97; 263 MB 62.7 -> 57.4 after other
 // work, 52.4 -> 57.1 where the step before had left them there; 137 MB 33.3 -> 36.7.
 constexpr std::uint64_t kStreamBytes = std::uint64_t(192) << 20;
-// Shared-out rows below which a head's pieces are added by all wavefronts of a
-// workgroup.
-constexpr unsigned kFewRows = 64;
+// Shared-out rows below which a head's pieces, 16 and more, are added by all
+// wavefronts of a workgroup (8 rows: 23.0 us, 29.5 with one wavefront per head; 4
+// rows, 54.1 -> 33.3), not by one (32 rows: 23.5 us, 21.9 with one; 64 rows: 35.3, 29.7).
+constexpr unsigned kFewRows = 32;
 // The fp16 form's probabilities are 2^(x - m + kBoost), m the running max less
 // at most kLazy: keys far below the max keep 10 more binary orders before they
 // become fp16 subnormals, and 2^(kBoost + kLazy) is far below fp16's largest.
@@ -141,8 +154,8 @@ __device__ __forceinline__ V fetch(const V* p) {
 // MT: 16-head operands per workgroup (group up to 16 MT). kPaged16: pages hold
 // whole 16-key blocks, so that a block's rows follow each other.
 // kStream: the cache is read past the caches' reach, with non-temporal loads.
-// kWideCap: fp16, capped in the precise form (one sequence of 65536 tokens 58.6 us
-// with it, 56.8 without).
+// kWideCap: fp16, capped in the precise form (two sequences of 131072 tokens 58.6 us
+// with it, 56.7 without).
 template <typename T, int DP, int MT, bool kPaged16, bool kStream, bool kWideCap>
 __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedArgs<T> a) {
   using S = Shape<T, DP>;
